@@ -480,6 +480,72 @@ int seera_sgd_step(float *w, const float *g, float *vel, int n, float lr, float 
 int seera_adam_step_dev(float *w, const float *g, float *m, float *v, int n, const float *hyper);
 int seera_sgd_step_dev(float *w, const float *g, float *vel, int n, const float *hyper);
 
+/* ---- layers over sequences and features --------------------------------------------------------------------------------
+ * No counterpart in the reference.  All of these may run inside batches and recordings; their scratch comes from the pool.
+ *
+ * Gated linear recurrence, per sequence n and channel c, with a = sigmoid(gate):
+ *     h[t] = a[t] h[t-1] + (1 - a[t]) cand[t],  h[-1] = h0
+ * `gate` and `cand` point at element [0, 0, 0] of their [N, T, C] columns; consecutive steps lie `ld` floats apart (>= C), consecutive
+ * sequences T * ld: two column ranges of one projection's output are such a pair.  h is [N, T, C], h0, h_last [N, C] (dense).
+ * lengths (N ints on the device, or NULL: all T; values outside 0..T are taken as the nearer of the two) ends a sequence early: its steps
+ * behind that are not read, h is 0 there and h_last is the state after the last step (h0 for a length of 0).
+ * h0 may be NULL (zeros); h or h_last may be NULL (not both), h_last may be h0 itself.  T = 1 is one step of decoding.
+ * Backward, from dh [N, T, C] and dh_last [N, C] (either may be NULL), with the h that the forward call wrote:
+ *     g[t] = dh[t] + c[t+1],  c[t] = a[t] g[t],  c[length] = dh_last;  dcand = (1 - a) g,  dgate = a (1 - a) (h[t-1] - cand[t]) g,  dh0 = c[0]
+ * dgate and dcand have steps `ld_grad` floats apart and are 0 behind a sequence's length; dh0 may be NULL.  No output may overlap an input
+ * (but h_last and h0).  The time axis is split where there are few sequences and channels: sums are taken in another order than step by step,
+ * the same one on every run. */
+int seera_gated_scan_fwd(const float *gate, const float *cand, int ld, const float *h0, const int *lengths, float *h, float *h_last, int N, int T,
+                         int C);
+int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const float *h0, const int *lengths, const float *h, const float *dh,
+                         const float *dh_last, float *dgate, float *dcand, int ld_grad, float *dh0, int N, int T, int C);
+/* Norms over the C features of each row (C <= 8192, else SEERA_E_LIMIT):  N(x) = (x - mu) / sqrt(mean((x - mu)^2) + eps), with mu the row's
+ * mean or, for SEERA_NORM_RMS, 0.
+ *     seera_norm_fwd   y = gamma N(x) + beta;  beta may be NULL; stats (rows x 2 floats, for the backward; 8-byte aligned) may be NULL
+ *     seera_norm_bwd   dx, dgamma, dbeta, each of which may be NULL
+ * What follows a block of a residual network, in one pass: the block's output u is normalised, gated and added to the scaled residual
+ * stream, and the next block's norm is taken of the sum:
+ *     out = scale res + act(gate) gamma N(u),   y = next_gamma N'(out) + next_beta
+ * gate has rows `ld_gate` floats apart and may be NULL (factor 1); act is one of SEERA_ACT_* (NONE: the gate as it is) or SEERA_ACT_SILU;
+ * res may be NULL (nothing added, scale is not read); y may be NULL (next_* is not used) and so may out if y is not; next_beta may be NULL.
+ * stats: rows x 4 floats for the backward (16-byte aligned), may be NULL.  y and out may each be u, res or a dense gate themselves (y may be x
+ * in seera_norm_fwd).
+ * Backward from dout and dy (either may be NULL, dy where the forward had no y): du, dgate (rows ld_dgate apart), dres, dgamma, dscale,
+ * dnext_gamma, dnext_beta, each of which may be NULL; out is formed anew and not needed.  Outputs must not overlap inputs.  Sums over the rows
+ * are taken in the same order on every run. */
+enum { SEERA_NORM_RMS = 0, SEERA_NORM_LAYER = 1 };
+enum { SEERA_ACT_SILU = 4 };          /* g * sigmoid(g); for gates */
+int seera_norm_fwd(const float *x, const float *gamma, const float *beta, float *y, float *stats, int rows, int C, int kind, float eps);
+int seera_norm_bwd(const float *dy, const float *x, const float *gamma, const float *stats, float *dx, float *dgamma, float *dbeta, int rows, int C,
+                   int kind);
+int seera_gated_residual_fwd(const float *u, const float *gate, int ld_gate, const float *res, const float *gamma, const float *scale, float *out,
+                             const float *next_gamma, const float *next_beta, float *y, float *stats, int rows, int C, int kind, int act,
+                             int next_kind, float eps, float next_eps);
+int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u, const float *gate, int ld_gate, const float *res, const float *gamma,
+                             const float *scale, const float *next_gamma, const float *stats, float *du, float *dgate, int ld_dgate, float *dres,
+                             float *dgamma, float *dscale, float *dnext_gamma, float *dnext_beta, int rows, int C, int kind, int act,
+                             int next_kind);
+/* AdamW over `count` tensors at once, in place (w, g, m, v, n, decay: host arrays of that length; n[i] entries, 0 allowed):
+ *     g' = grad_scale g;  m = beta1 m + omb1 g';  v = beta2 v + omb2 g'^2;  w = (1 - lr decay) w - lr (m / c1) / (sqrt(v / c2) + eps)
+ * with the scalars of seera_adam_step and one decay per tensor.  Where `hyper` (device memory) is not NULL the scalars are read from there
+ * at run time, in the order of the arguments.  In a recording without `hyper`, seera_graph_set_scalars replaces them (9 floats, 10 in 8 bits).
+ * The tensors must not overlap.
+ * seera_adamw8_step holds m and v in 8 bits: `state` of a tensor is seera_adamw8_state_bytes(n) bytes (8-byte aligned; zeros to start
+ * with), 136 for each 64 neighbouring entries: sixteen times four codes of m and four of v, then the largest |m| and the largest v of the 64 as
+ * floats.  A code times the block's largest is the entry: m has a sign, 4 bits of exponent and 3 of mantissa, v 5 bits of exponent and 3 of mantissa.
+ * Rounding goes up or down at random with the value as its mean; the random bits follow from `step` (the number of the step, a whole number below 2^24)
+ * and the entry's place: `first` plus its place in the tensors one after the other, each rounded up to 64.  w is updated from m and v before they are
+ * rounded.  An infinity or a NaN in a gradient makes the m and v of its 64 entries NaN, where 32 bits would keep it to the one.
+ * seera_adamw8_read writes out the m and v that a state of n entries stands for. */
+int seera_adamw_step(int count, float *const *w, const float *const *g, float *const *m, float *const *v, const long long *n, const float *decay,
+                     float lr, float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale,
+                     const float *hyper);
+size_t seera_adamw8_state_bytes(long long n);
+int seera_adamw8_step(int count, float *const *w, const float *const *g, void *const *state, const long long *n, const float *decay, float lr,
+                      float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale, float step,
+                      const float *hyper, long long first);
+int seera_adamw8_read(const void *state, float *m, float *v, long long n);
+
 /* ---- data parallel: the gradient exchange of a batch sharded over the GPUs of one node -----------------------------
  * No counterpart in the reference (single GPU only).  One process per GPU; every rank holds the same weights and
  * trains its shard; the weight-gradient arena is summed over the ranks with NCCL over NVLink / NVSwitch and the

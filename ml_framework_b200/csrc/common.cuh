@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 #include <cstdio>
+#include <memory>
 #include "seera_b200.h"
 
 namespace seera {
@@ -135,10 +136,12 @@ struct ProfBytes {
 // An optimizer launch, described so that a recorded one can be given other scalars (runtime.cu, fused.cu).
 struct OptLaunch {
     static constexpr int MAX_ARGS = 16;
-    int kind;                      // 0 Adam, 1 SGD
+    int kind;                      // 0 Adam, 1 SGD, 2 AdamW
     float *w; const float *g; float *m, *v;
     long long n; bool vec; int grid;
-    float scalars[9]; int n_scalars;
+    float scalars[10]; int n_scalars;
+    const void *func;              // AdamW: the kernel and the table of its tensors, its arguments in front of the scalars
+    std::shared_ptr<void> table;
 };
 int graph_note_optimizer(const OptLaunch &launch);
 void graph_note_launch(const void *func, dim3 grid, dim3 block, size_t smem);

@@ -488,6 +488,12 @@ __global__ void __launch_bounds__(256) sgd_kernel(float *__restrict__ w, const f
 void optimizer_node_params(const OptLaunch &l, cudaKernelNodeParams &kp, void **args) {
     OptLaunch *o = const_cast<OptLaunch *>(&l);
     int i = 0;
+    if (l.kind == 2) {
+        args[0] = o->table.get(); args[1] = o->scalars;
+        kp.func = const_cast<void *>(l.func);
+        kp.gridDim = dim3(l.grid); kp.blockDim = dim3(256); kp.sharedMemBytes = 0; kp.kernelParams = args; kp.extra = nullptr;
+        return;
+    }
     args[i++] = &o->w; args[i++] = &o->g; args[i++] = &o->m;
     if (l.kind == 0) args[i++] = &o->v;
     args[i++] = &o->n; args[i++] = &o->vec;

@@ -11,6 +11,7 @@
 #include <utility>
 #include <pybind11/stl.h>
 
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -21,6 +22,8 @@ namespace py = pybind11;
 using arr_f = py::array_t<float, py::array::c_style | py::array::forcecast>;
 using arr_i = py::array_t<int32_t, py::array::c_style | py::array::forcecast>;
 using arr_s = py::array_t<int16_t, py::array::c_style | py::array::forcecast>;
+using arr_p = py::array_t<uint64_t, py::array::c_style | py::array::forcecast>;
+using arr_l = py::array_t<long long, py::array::c_style | py::array::forcecast>;
 using uptr = uintptr_t;
 
 static inline void ck(int status) {
@@ -32,6 +35,12 @@ static inline uptr ckp(void *p) {
 }
 template <class T> static inline T *P(uptr a) { return reinterpret_cast<T *>(a); }
 using F = float;
+
+static py::ssize_t same_length(std::initializer_list<py::ssize_t> sizes) {
+    for (py::ssize_t k : sizes)
+        if (k != *sizes.begin()) throw std::runtime_error("[seera_cuda] one entry per tensor in each array");
+    return *sizes.begin();
+}
 
 template <class T, class Arr>
 static Arr download(uptr ptr, const py::tuple &shape) {
@@ -186,6 +195,43 @@ PYBIND11_MODULE(seera_cuda, m) {
     m.def("batches_kept", []() { return seera_batches_kept(); });
     m.def("graph_set_scalars", [](uptr g, const std::vector<float> &v) { ck(seera_graph_set_scalars(P<void>(g), v.data(), (int)v.size())); });
     m.def("is_capturing", []() { return seera_is_capturing() != 0; });
+    // ---- layers over sequences and features ----------------------------------------------------------
+    m.def("gated_scan_fwd", [](uptr f, uptr v, int ld, uptr h0, uptr len, uptr h, uptr last, int N, int T, int C) {
+        ck(seera_gated_scan_fwd(P<const F>(f), P<const F>(v), ld, P<const F>(h0), P<const int>(len), P<F>(h), P<F>(last), N, T, C)); });
+    m.def("gated_scan_bwd", [](uptr f, uptr v, int ld, uptr h0, uptr len, uptr h, uptr dh, uptr dlast, uptr df, uptr dv, int ldg, uptr dh0, int N, int T, int C) {
+        ck(seera_gated_scan_bwd(P<const F>(f), P<const F>(v), ld, P<const F>(h0), P<const int>(len), P<const F>(h), P<const F>(dh), P<const F>(dlast),
+                                P<F>(df), P<F>(dv), ldg, P<F>(dh0), N, T, C)); });
+    m.def("norm_fwd", [](uptr x, uptr g, uptr b, uptr y, uptr st, int rows, int C, int kind, float eps) {
+        ck(seera_norm_fwd(P<const F>(x), P<const F>(g), P<const F>(b), P<F>(y), P<F>(st), rows, C, kind, eps)); });
+    m.def("norm_bwd", [](uptr dy, uptr x, uptr g, uptr st, uptr dx, uptr dg, uptr db, int rows, int C, int kind) {
+        ck(seera_norm_bwd(P<const F>(dy), P<const F>(x), P<const F>(g), P<const F>(st), P<F>(dx), P<F>(dg), P<F>(db), rows, C, kind)); });
+    m.def("gated_residual_fwd", [](uptr u, uptr gate, int ldg, uptr res, uptr ga, uptr sc, uptr out, uptr g2, uptr b2, uptr y, uptr st, int rows, int C,
+                                   int kind, int act, int kind2, float eps, float eps2) {
+        ck(seera_gated_residual_fwd(P<const F>(u), P<const F>(gate), ldg, P<const F>(res), P<const F>(ga), P<const F>(sc), P<F>(out), P<const F>(g2),
+                                    P<const F>(b2), P<F>(y), P<F>(st), rows, C, kind, act, kind2, eps, eps2)); });
+    m.def("gated_residual_bwd", [](uptr dout, uptr dy, uptr u, uptr gate, int ldg, uptr res, uptr ga, uptr sc, uptr g2, uptr st, uptr du, uptr dgate, int lddg,
+                                   uptr dres, uptr dga, uptr dsc, uptr dg2, uptr db2, int rows, int C, int kind, int act, int kind2) {
+        ck(seera_gated_residual_bwd(P<const F>(dout), P<const F>(dy), P<const F>(u), P<const F>(gate), ldg, P<const F>(res), P<const F>(ga), P<const F>(sc),
+                                    P<const F>(g2), P<const F>(st), P<F>(du), P<F>(dgate), lddg, P<F>(dres), P<F>(dga), P<F>(dsc), P<F>(dg2), P<F>(db2),
+                                    rows, C, kind, act, kind2)); });
+    // Host arrays, one entry per tensor: addresses, numbers of entries, decays.
+    m.def("adamw_step", [](arr_p w, arr_p g, arr_p mm, arr_p v, arr_l n, arr_f decay, float lr, float b1, float omb1, float b2, float omb2, float eps, float c1,
+                           float c2, float gs, uptr hyper) {
+        const py::ssize_t k = same_length({w.size(), g.size(), mm.size(), v.size(), n.size(), decay.size()});
+        ck(seera_adamw_step((int)k, (F *const *)w.data(), (const F *const *)g.data(), (F *const *)mm.data(), (F *const *)v.data(), n.data(), decay.data(),
+                            lr, b1, omb1, b2, omb2, eps, c1, c2, gs, P<const F>(hyper)));
+    }, py::arg("w"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("n"), py::arg("decay"), py::arg("lr"), py::arg("beta1"), py::arg("omb1"), py::arg("beta2"),
+       py::arg("omb2"), py::arg("eps"), py::arg("c1"), py::arg("c2"), py::arg("grad_scale"), py::arg("hyper") = 0);
+    m.def("adamw8_state_bytes", [](long long n) { return seera_adamw8_state_bytes(n); });
+    m.def("adamw8_step", [](arr_p w, arr_p g, arr_p st, arr_l n, arr_f decay, float lr, float b1, float omb1, float b2, float omb2, float eps, float c1, float c2,
+                            float gs, float step, uptr hyper, long long first) {
+        const py::ssize_t k = same_length({w.size(), g.size(), st.size(), n.size(), decay.size()});
+        ck(seera_adamw8_step((int)k, (F *const *)w.data(), (const F *const *)g.data(), (void *const *)st.data(), n.data(), decay.data(), lr, b1, omb1, b2,
+                             omb2, eps, c1, c2, gs, step, P<const F>(hyper), first));
+    }, py::arg("w"), py::arg("g"), py::arg("state"), py::arg("n"), py::arg("decay"), py::arg("lr"), py::arg("beta1"), py::arg("omb1"), py::arg("beta2"),
+       py::arg("omb2"), py::arg("eps"), py::arg("c1"), py::arg("c2"), py::arg("grad_scale"), py::arg("step"), py::arg("hyper") = 0, py::arg("first") = 0);
+    m.def("adamw8_read", [](uptr st, uptr mm, uptr v, long long n) { ck(seera_adamw8_read(P<const void>(st), P<F>(mm), P<F>(v), n)); });
+
     m.def("cuda_adam_step_dev", [](uptr w, uptr g, uptr mm, uptr v, int n, uptr h) {
         ck(seera_adam_step_dev(P<F>(w), P<const F>(g), P<F>(mm), P<F>(v), n, P<const F>(h))); });
     m.def("cuda_sgd_step_dev", [](uptr w, uptr g, uptr vel, int n, uptr h) {
