@@ -98,6 +98,7 @@ class Tensor:
     _copies = None                   # channels-last copies of the value, made by its producer for a convolution
     _rows = None                     # row-major copies of the value, made by its producer for a Dense layer
     _pass = None                     # (input shape, reference to the model) of the pass it came from
+    _gate = None                     # a GatedRecurrence's output: the _OutputGate beside it
 
     def __init__(self, value, dtype="float32", is_leaf=False, device="cuda"):
         if isinstance(value, Tensor):
@@ -144,10 +145,15 @@ class Tensor:
         return _new(self.value.shape)
 
     def _accumulate(self, g):
-        """Add a gradient contribution: a cuten of this tensor's shape, or a _PooledGrad (the gradient of a 2x2 max-pool
-        of this tensor, still in pooled form) when it is the only contribution."""
+        """Add a gradient contribution: a cuten of this tensor's shape, a _PooledGrad (the gradient of a 2x2 max-pool
+        of this tensor, still in pooled form) when it is the only contribution, or a _NormGrad."""
         if self.grad is None:
             self.grad = g
+        elif g.__class__ is _NormGrad:
+            g.add(self.grad)
+            self.grad = g
+        elif self.grad.__class__ is _NormGrad:
+            self.grad.add(g)
         else:
             if isinstance(self.grad, _PooledGrad):
                 self.grad = self.grad.materialize()
@@ -219,6 +225,32 @@ class _PooledGrad:
         return dx
 
 
+class _NormGrad:
+    """Gradient of a tensor of which a norm over the features has been taken: `dy`, that of the norm's output, with the `norm` layer and the
+    `plain` gradient that came over other ways (or None).  The layer that took the norm in its own launch (GatedResidual) also goes back through it in
+    its own."""
+    __slots__ = ("dy", "norm", "plain")
+
+    def __init__(self, dy, norm):
+        self.dy, self.norm, self.plain = dy, norm, None
+
+    def add(self, g):
+        if self.plain is not None:
+            out = _new(g.shape)
+            sc.cuda_elemadd(self.plain.main_ptr, g.main_ptr, out.main_ptr, g.size)
+            g = out
+        self.plain = g
+
+
+class _OutputGate:
+    """The third range of columns of a GatedRecurrence's projection: the gate that the next layer puts on its output.  `grad`, as wide as the
+    projection, is where that layer leaves the gate's gradient."""
+    __slots__ = ("z", "units", "grad", "taken")
+
+    def __init__(self, z, units):
+        self.z, self.units, self.grad, self.taken = z, units, None, False
+
+
 class _Formed(cuten):
     """A tensor whose values are formed from another's when its address is asked for.  One that is left unformed by a recording is formed
     anew each time it is asked for: every replay changes what it is formed from."""
@@ -279,6 +311,11 @@ class _Softmax(_Formed):
 
     def _form(self):
         sc.cuda_softmax_fwd(self.source.main_ptr, self._ptr, *self.shape)
+
+
+# A norm over the features behind a GatedResidual runs in that layer's launch, in both directions: forward 20 bytes an element instead of 24,
+# backward 32 instead of 44.  Set to False to give every norm a launch of its own.
+FUSE_NORM = True
 
 
 class _KeptCopies:
@@ -378,6 +415,8 @@ class Layer:
     _pool_consumer = None
     _feeds_conv = _feeds_dense = _feeds_convT = _feeds_copies = False
     _fused = None                    # a pool that the layer folded into its own launch: (pooled, mask, copies)
+    _norm_consumer = None            # the norm layer behind a GatedResidual
+    _normed = None                   # ... and that norm's output, where that layer made it in its own launch: (layer, values)
     _model = None
 
     def __init__(self):
@@ -959,8 +998,274 @@ class Flatten(Layer):
         return "Flatten Layer"
 
 
+# ---- layers over sequences and features ------------------------------------------------------------------------------------------
+_NORMS = {"rms": 0, "layer": 1}
+_GATES = {None: 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4}
+
+
+def _rescale_gradients(g):
+    """Behind a layer whose gradient may be larger than the loss's by any factor (a norm divides by its row's size) the fp16 precision modes
+    take the factor of their gradient copies anew."""
+    if sc.get_precision() in (4, 5):
+        sc.grad_scale_update(g.main_ptr, g.size)
+
+
+def _rows_of(layer, shape, units):
+    if len(shape) < 2 or shape[-1] != units:
+        raise ValueError(f"{layer} expects (..., {units}), got {tuple(shape)}")
+    return _numel(shape[:-1])
+
+
+class _FeatureNorm(_ParamLayer):
+    """gamma N(x) + beta over the last axis of a tensor of two or more; gamma / beta are the layer's `weights` / `bais`.  Behind a GatedResidual
+    of as many units it runs in that layer's launches."""
+    kind = "rms"
+
+    def __init__(self, units, eps):
+        super().__init__()
+        self.units, self.eps = int(units), float(eps)
+        self._w_init = np.ones((self.units,), np.float32)
+        self._b_init = np.zeros((self.units,), np.float32)
+        self.weights = Tensor(self._w_init, is_leaf=True)
+        self.bais = Tensor(self._b_init, is_leaf=True)
+
+    gamma = property(lambda self: self.weights)
+    beta = property(lambda self: self.bais)
+
+    def __call__(self, input_layer):
+        super().__call__(input_layer)
+        if isinstance(input_layer, GatedResidual) and input_layer.units == self.units:
+            input_layer._norm_consumer = weakref.ref(self)
+        return self
+
+    def forward(self):
+        x = self.inputs = self.inpobj.outputs
+        xv = x.value
+        shape = xv.shape
+        rows, C, kind = _rows_of(self, shape, self.units), self.units, _NORMS[self.kind]
+        g, b = self.weights, self.bais
+        made = self.inpobj._normed
+        if made is not None and made[0] is self:  # the layer before has made it, and its gradients will be formed there too
+            self.inpobj._normed = None
+            owner = self._model
+            self.outputs = out = Tensor._of(made[1], (x, g, b), lambda dy: x._accumulate(_NormGrad(dy, (g, b, owner))))
+            return out
+        y, stats = _new(shape), _new((rows, 2))
+        sc.norm_fwd(xv.main_ptr, g.value.main_ptr, b.value.main_ptr, y._ptr, stats._ptr, rows, C, kind, self.eps)
+        need_dx, owner = not x.is_leaf, self._model
+
+        def backward(dy):
+            dg, db = g._grad_target(), b._grad_target()
+            dx = _new(shape) if need_dx else None
+            sc.norm_bwd(dy.main_ptr, xv.main_ptr, g.value._ptr, stats._ptr, dx._ptr if need_dx else 0, dg._ptr, db._ptr, rows, C, kind)
+            if need_dx:
+                _rescale_gradients(dx)
+            _deliver(owner, x, g, b, dx, dg, db)
+        self.outputs = out = Tensor._of(y, (x, g, b), backward)
+        return out
+
+    def __repr__(self):
+        return f"{self.__class__.__name__}({self.units})"
+
+
+class RMSNorm(_FeatureNorm):
+    """x / sqrt(mean(x^2) + eps) * gamma + beta over the last axis."""
+
+    def __init__(self, units, eps=1e-6):
+        super().__init__(units, eps)
+
+
+class LayerNorm(_FeatureNorm):
+    """(x - mean(x)) / sqrt(var(x) + eps) * gamma + beta over the last axis."""
+    kind = "layer"
+
+    def __init__(self, units, eps=1e-5):
+        super().__init__(units, eps)
+
+
+class GatedRecurrence(_ParamLayer):
+    """Gated linear recurrence over the time axis of (N, T, in_units): the columns of z = x W + b are gate logits f and candidates v, and
+    h[t] = a[t] h[t-1] + (1 - a[t]) v[t] with a = sigmoid(f), from a state of zeros.  W is (in_units, 2 units).
+
+    output_gate       W has a third range of columns, which a GatedResidual behind this layer takes as the gate of what it adds.
+    return_sequences  the output is (N, T, units), every h; else (N, units), the last.
+    stateful          `predict` goes on from the state that the `predict` before it left, until reset_states(): token by token, or a long
+                      sequence in parts.  Training passes always start from zeros.
+    Sequences shorter than T: `Sequential.forward(X, lengths=...)`.  Steps behind a sequence's length are not read and give zeros; the last h is that
+    of its last step."""
+
+    def __init__(self, in_units, units, output_gate=False, return_sequences=True, stateful=False, kernel_initializer="glorot_uniform",
+                 bias_initializer="zeros"):
+        super().__init__()
+        if output_gate and not return_sequences:
+            raise ValueError("an output gate goes with every step: return_sequences=True")
+        table = _initializers(in_units, units)
+        for initializer in (kernel_initializer, bias_initializer):
+            if initializer not in table:
+                raise ValueError(f"Initializer must be one of {list(table.keys())}")
+        self.in_units, self.units, self.output_gate = int(in_units), int(units), bool(output_gate)
+        self.return_sequences, self.stateful, self.training, self._state = bool(return_sequences), bool(stateful), True, None
+        self._cols = (3 if output_gate else 2) * self.units
+        self._w_init = _initial(table[kernel_initializer], (self.in_units, self._cols))
+        self._b_init = _initial(table[bias_initializer], (1, self._cols))
+        self.weights = Tensor(self._w_init, is_leaf=True)
+        self.bais = Tensor(self._b_init, is_leaf=True)
+
+    def reset_states(self):
+        """The next `predict` starts from zeros again."""
+        self._state = None
+
+    def forward(self):
+        x = self.inputs = self.inpobj.outputs
+        W, b = self.weights, self.bais
+        xv, wv = x.value, W.value
+        shape = xv.shape
+        if len(shape) != 3 or shape[2] != self.in_units:
+            raise ValueError(f"{self} expects (N, T, {self.in_units}), got {tuple(shape)}")
+        N, T, K = shape
+        U, cols, M = self.units, self._cols, N * T
+        model = self._model and self._model()
+        lengths = model._lengths if model is not None else None
+        if lengths is not None and lengths.size != N:
+            raise ValueError(f"{lengths.size} lengths for {N} sequences")
+        state = None
+        if self.stateful and not self.training:
+            if self._state is None:
+                if sc.is_capturing():
+                    raise RuntimeError("a recording goes on from a state: predict once before it")
+                self._state = _wrap(sc.cuda_zeros_f(N * U), (N, U))
+            state = self._state
+            if state.shape != (N, U):
+                raise ValueError(f"the state is that of {state.shape[0]} sequences, the input has {N}: reset_states() first")
+        z = _new((N, T, cols))
+        ha, hw, _ = sc.matmul_bias_act_fwd_s(xv.main_ptr, wv.main_ptr, b.value.main_ptr, z._ptr, M, cols, K, 0, 0, False)
+        kept_a, kept_w = _KeptRows(ha) if ha else None, _KeptRows(hw) if hw else None
+        whole = self.return_sequences
+        h = _new((N, T, U)) if whole or self.training else None
+        last = state if state is not None else (None if whole else _new((N, U)))
+        at = lambda t: 0 if t is None else t.main_ptr  # noqa: E731
+        sc.gated_scan_fwd(z._ptr, z._ptr + 4 * U, cols, at(state), at(lengths), at(h), at(last), N, T, U)
+        if not whole and state is not None:                 # the output is a tensor of its own: the next call writes the state
+            last = _new((N, U))
+            sc.cuda_memcopy_devicetodevice(last._ptr, state.main_ptr, N * U)
+        gate = _OutputGate(z, U) if self.output_gate else None
+        need_dx, owner, carried = not x.is_leaf, self._model, state is not None or h is None
+
+        def backward(g):
+            if carried:
+                raise RuntimeError("a prediction of a GatedRecurrence with a state carried on, or of its last step alone, has no gradient: use forward()")
+            dz = gate.grad if gate is not None else None
+            if dz is None:
+                dz = _new((N, T, cols))
+                if gate is not None:                        # nobody took the gate
+                    sc.cuda_memset(dz._ptr, 0, 4 * M * cols)
+            else:
+                gate.grad = None
+            sc.gated_scan_bwd(z._ptr, z._ptr + 4 * U, cols, 0, at(lengths), h._ptr, g.main_ptr if whole else 0, 0 if whole else g.main_ptr,
+                              dz._ptr, dz._ptr + 4 * U, cols, 0, N, T, U)
+            _rescale_gradients(dz)
+            db, dw = b._grad_target(), W._grad_target()
+            dx = _new(shape) if need_dx else None
+            sc.matmul_act_bwd(xv.main_ptr, wv._ptr, 0, dz._ptr, dx._ptr if need_dx else 0, dw._ptr, db._ptr, M, cols, K, 0,
+                              kept_a.h if kept_a else 0, kept_w.h if kept_w else 0)
+            for k in (kept_a, kept_w):
+                if k:
+                    k.release()
+            _deliver(owner, x, W, b, dx, dw, db)
+        self.outputs = out = Tensor._of(h if whole else last, (x, W, b), backward)
+        out._gate = gate
+        return out
+
+    def __repr__(self):
+        return f"GatedRecurrence({self.in_units}→{self.units}{', output gate' if self.output_gate else ''})"
+
+
+class GatedResidual(_ParamLayer):
+    """The end of a block: out = scale * residual + act(gate) * gamma * N(u), u the output of the layer before.
+
+    residual    the layer whose output is added (one before this in the model), or None
+    activation  of the gate: "silu", "sigmoid", "tanh", "relu" or None (the gate as it is).  The gate is the output gate of a GatedRecurrence right
+                before this layer; where there is none the factor is 1.
+    norm        "rms" or "layer"
+    gamma / scale are the layer's `weights` / `bais`, both ones to begin with.  A norm layer of as many units behind this one is taken in the same launch."""
+
+    def __init__(self, units, residual=None, activation="silu", norm="rms", eps=1e-6):
+        super().__init__()
+        if activation not in _GATES:
+            raise ValueError('Activation must be "relu", "sigmoid", "tanh", "silu" or None')
+        if norm not in _NORMS:
+            raise ValueError('Norm must be "rms" or "layer"')
+        if residual is not None and not isinstance(residual, Layer):
+            raise TypeError("The residual should be a Layer")
+        self.units, self.residual, self.activation, self.norm, self.eps = int(units), residual, activation, norm, float(eps)
+        self._w_init = np.ones((self.units,), np.float32)
+        self._b_init = np.ones((self.units,), np.float32)
+        self.weights = Tensor(self._w_init, is_leaf=True)
+        self.bais = Tensor(self._b_init, is_leaf=True)
+
+    gamma = property(lambda self: self.weights)
+    scale = property(lambda self: self.bais)
+
+    def forward(self):
+        u = self.inputs = self.inpobj.outputs
+        r = None if self.residual is None else self.residual.outputs
+        uv = u.value
+        shape = uv.shape
+        rows, C = _rows_of(self, shape, self.units), self.units
+        if r is not None and tuple(r.value.shape) != tuple(shape):
+            raise ValueError(f"{self}: residual of {tuple(r.value.shape)} beside {tuple(shape)}")
+        gate = u._gate
+        if gate is not None:
+            if gate.taken:
+                raise ValueError("an output gate is read by one layer")
+            gate.taken = True
+        kind, act, g, b = _NORMS[self.norm], _GATES[self.activation], self.weights, self.bais
+        norm = FUSE_NORM and self._norm_consumer and self._norm_consumer()
+        kind2, eps2 = (_NORMS[norm.kind], norm.eps) if norm else (0, 0.0)
+        out, y, stats = _new(shape), _new(shape) if norm else None, _new((rows, 4))
+        pg, ld = (gate.z.main_ptr + 8 * C, 3 * C) if gate is not None else (0, 0)
+        rv = None if r is None else r.value
+        sc.gated_residual_fwd(uv.main_ptr, pg, ld, rv.main_ptr if rv is not None else 0, g.value.main_ptr, b.value.main_ptr, out._ptr,
+                              norm.weights.value.main_ptr if norm else 0, norm.bais.value.main_ptr if norm else 0, y._ptr if norm else 0,
+                              stats._ptr, rows, C, kind, act, kind2, self.eps, eps2)
+        self._normed = (norm, y) if norm else None
+        need_du, need_dr, owner = not u.is_leaf or gate is not None, r is not None and not r.is_leaf, self._model
+
+        def backward(grad):
+            dy = None
+            dout = grad
+            if grad.__class__ is _NormGrad:
+                dy, dout = grad.dy, grad.plain
+                ng, nb, nowner = grad.norm
+                dng, dnb = ng._grad_target(), nb._grad_target()
+            dg, db = g._grad_target(), b._grad_target()
+            du, dr = _new(shape) if need_du else None, _new(shape) if need_dr else None
+            if gate is not None:
+                gate.grad = _new(gate.z.shape)
+            sc.gated_residual_bwd(dout.main_ptr if dout is not None else 0, dy.main_ptr if dy is not None else 0, uv.main_ptr, pg, ld,
+                                  rv.main_ptr if rv is not None else 0, g.value._ptr, b.value._ptr, ng.value._ptr if dy is not None else 0, stats._ptr,
+                                  du._ptr if need_du else 0, gate.grad._ptr + 8 * C if gate is not None else 0, ld, dr._ptr if need_dr else 0,
+                                  dg._ptr, db._ptr if rv is not None else 0, dng._ptr if dy is not None else 0, dnb._ptr if dy is not None else 0,
+                                  rows, C, kind, act, kind2)
+            if rv is None:
+                sc.cuda_memset(db.main_ptr, 0, 4 * C)
+            if need_du:
+                _rescale_gradients(du)
+            if dy is not None:
+                _deliver(nowner, None, ng, nb, None, dng, dnb)
+            if need_dr:
+                r._accumulate(dr)
+            _deliver(owner, u, g, b, du if not u.is_leaf else None, dg, db)
+        parents = (u, g, b) if r is None else (u, r, g, b)
+        self.outputs = t = Tensor._of(out, parents, backward)
+        return t
+
+    def __repr__(self):
+        return f"GatedResidual({self.units}, gate={self.activation}, norm={self.norm})"
+
+
 _OWN_LAYERS = {c: c.forward for c in (Input, Dense, Conv2D, ConvTranspose2D, BatchNorm1d, BatchNorm2d, Concatenate, MaxPool2D, Unpool2D_Nearest,
-                                       Flatten)}
+                                       Flatten, RMSNorm, LayerNorm, GatedRecurrence, GatedResidual)}
 
 
 # ─────────────────────────────────────────────────────────────────────────────────────────────
@@ -976,7 +1281,7 @@ def _train_step(model, optimizer, lossf, y):
 
 
 def _own_step(optimizer, lossf):
-    return optimizer.__class__ in (SGD, Adam) and getattr(lossf, "__func__", None) in _LOSSES
+    return optimizer.__class__ in (SGD, Adam, AdamW) and getattr(lossf, "__func__", None) in _LOSSES
 
 
 # Full batches left to run from which recording the step pays: recording costs the host an eager step, a replay half of one (small CNN
@@ -1030,6 +1335,7 @@ class _RecordedStep:
 
 class Sequential:
     _whole = False                   # in predict: a softmax that the last layer's launch can form is formed there
+    _lengths = None                  # of the current pass's sequences, on the device
 
     def __init__(self, layers, device="cuda"):
         if not isinstance(layers, list):
@@ -1040,6 +1346,9 @@ class Sequential:
             raise ValueError("this engine has no CPU path: Sequential(..., device=\"cuda\")")
         self.device = device
         self.model = [layers[0]] + [layer(layers[i]) for i, layer in enumerate(layers[1:])]
+        for i, l in enumerate(self.model):
+            if isinstance(l, GatedResidual) and l.residual is not None and not any(l.residual is k for k in self.model[:i]):
+                raise ValueError(f"the residual of {l} is not a layer before it in the model")
         self.world, self._allreduce, self._on_grad_ready = 1, None, None
         self._modal = [l for l in self.model if hasattr(l, "training")]       # layers that behave differently in evaluation
         self._passes = set()                          # kinds and sizes of passes made (see _open_batch)
@@ -1092,13 +1401,25 @@ class Sequential:
     def parameters(self):
         return [t for l in self.param_layers for t in (l.weights, l.bais)]
 
-    def forward(self, X=None):
+    def forward(self, X=None, lengths=None):
+        """`lengths`: how many steps each sequence of an (N, T, ...) input has, for the layers that go through time: host integers or a
+        device tensor of int32."""
         if X is not None:
             if isinstance(X, np.ndarray):
                 X = Tensor(X, is_leaf=True)
             if not isinstance(X, Tensor):
                 raise TypeError("Input must be a Tensor or numpy array.")
             self.model[0].inputs = X
+        if lengths is not None and not isinstance(lengths, cuten):
+            if sc.is_capturing():
+                raise RuntimeError("a recording takes its lengths from a device tensor")
+            lengths = np.asarray(lengths)
+            if lengths.ndim != 1 or not np.issubdtype(lengths.dtype, np.integer):
+                raise ValueError("lengths should be one integer per sequence")
+            lengths = cuten(lengths.astype(np.int32), "int32")
+        if lengths is not None and (lengths.dtype != "int32" or lengths.size != self.model[0].inputs.value.shape[0]):
+            raise ValueError(f"{lengths.size} lengths of {lengths.dtype} for {self.model[0].inputs.value.shape[0]} sequences (int32)")
+        self._lengths = lengths
         size = None
         if _inside.n:                                 # part of a training step's, whose first part ends with the forward
             _batch_begin(_STEP)
@@ -1136,12 +1457,13 @@ class Sequential:
             return False
         return True
 
-    def predict(self, X):
-        """Forward in evaluation mode: BatchNorm layers normalise with their running statistics (Seera.py:690-700)."""
+    def predict(self, X, lengths=None):
+        """Forward in evaluation mode: BatchNorm layers normalise with their running statistics (Seera.py:690-700), a GatedRecurrence with
+        a state goes on from it."""
         self._set_mode(False)
         self._whole = True
         try:
-            return self.forward(X)
+            return self.forward(X) if lengths is None else self.forward(X, lengths)
         finally:
             self._whole = False
             self._set_mode(True)
@@ -1329,6 +1651,14 @@ class Sequential:
                                   "eps": l.eps, "running_mean": l.running_mean, "running_var": l.running_var}
             elif isinstance(l, Unpool2D_Nearest):
                 info["config"] = {"size": l.size}
+            elif isinstance(l, _FeatureNorm):
+                info["config"] = {"units": l.units, "eps": l.eps}
+            elif isinstance(l, GatedRecurrence):
+                info["config"] = {"in_units": l.in_units, "units": l.units, "output_gate": l.output_gate, "return_sequences": l.return_sequences,
+                                  "stateful": l.stateful}
+            elif isinstance(l, GatedResidual):
+                info["config"] = {"units": l.units, "activation": l.activation, "norm": l.norm, "eps": l.eps,
+                                  "residual": None if l.residual is None else [k is l.residual for k in self.model].index(True)}
             if isinstance(l, _ParamLayer):
                 info["weights"], info["bais"] = l.weights.to_numpy(), l.bais.to_numpy()
             data.append(info)
@@ -1369,6 +1699,12 @@ class Sequential:
                 l = Flatten()
             elif k == "Concatenate":
                 l = Concatenate()
+            elif k in ("RMSNorm", "LayerNorm"):
+                l = (RMSNorm if k == "RMSNorm" else LayerNorm)(c["units"], c["eps"])
+            elif k == "GatedRecurrence":
+                l = GatedRecurrence(**c)
+            elif k == "GatedResidual":
+                l = GatedResidual(**{**c, "residual": None if c["residual"] is None else layers[c["residual"]]})
             else:
                 raise ValueError(f"Unknown layer type: {k}")
             if "weights" in info:
@@ -1489,6 +1825,11 @@ class _Optimizer:
             o = Adam(model, lr=state["lr"], beta1=state["beta1"], beta2=state["beta2"], eps=state["eps"])
             o.t = state["t"]
             arenas = (("m", o.m), ("v", o.v))
+        elif state["kind"] == "adamw":
+            o = AdamW(model, lr=state["lr"], beta1=state["beta1"], beta2=state["beta2"], eps=state["eps"], weight_decay=state["weight_decay"],
+                      state_bits=state["state_bits"])
+            o.t = state["t"]
+            arenas = (("m", o.m), ("v", o.v)) if o.state_bits == 32 else (("state", o.state),)
         else:
             o = SGD(model, lr=state["lr"], momentum=state["momentum"])
             arenas = (("velocity", o.velocity),)
@@ -1587,3 +1928,67 @@ class Adam(_Optimizer):
             sc.cuda_adam_step_dev(*at, self._hyper.main_ptr)
         else:
             sc.cuda_adam_step(*at, *scalars)
+
+
+class AdamW(_Optimizer):
+    """Adam with decoupled weight decay: w = (1 - lr weight_decay) w - lr (m / c1) / (sqrt(v / c2) + eps).  The layers' weight matrices and
+    filters decay; biases and the factors of norms do not.  A recorded step keeps the weight_decay that it was recorded with (lr and the rest follow).
+
+    state_bits  32, or 8: m and v in 8 bits each with a largest value per 64 entries, 2.125 bytes a parameter instead of 8 (see seera_adamw8_step)."""
+
+    def __init__(self, model, lr=0.001, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32):
+        super().__init__(model)
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits should be 8 or 32")
+        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.state_bits, self.t = lr, beta1, beta2, eps, weight_decay, state_bits, 1
+        if state_bits == 32:
+            self.m, self.v = self._state(), self._state()
+        else:
+            n = max(sc.adamw8_state_bytes(model.n_arena) // 4, 2)
+            self.state = cuten._wrap(sc.cuda_zeros_f(n), (n,))
+        ps = model.parameters()
+        self._offs = np.array([p._arena_off for p in ps], np.uint64)
+        self._n = np.array([p._arena_n for p in ps], np.int64)
+        self._matrix = np.array([t is l.weights and len(t.value.shape) > 1 for l in model.param_layers for t in (l.weights, l.bais)], bool)
+        self._tables = {}
+
+    def _scalars(self, count=True):
+        """The update's scalars at the current step; `count` moves on to the next step."""
+        b1, b2, t = self.beta1, self.beta2, self.t
+        if count:
+            self.t = t + 1
+        s = [self.lr, b1, 1 - b1, b2, 1 - b2, self.eps, 1 - b1 ** t, 1 - b2 ** t, self._grad_scale()]
+        return s if self.state_bits == 32 else s + [float(t)]
+
+    def state_dict(self):
+        d = {"kind": "adamw", "lr": self.lr, "beta1": self.beta1, "beta2": self.beta2, "eps": self.eps, "weight_decay": self.weight_decay,
+             "state_bits": self.state_bits, "t": self.t}
+        for name in ("m", "v") if self.state_bits == 32 else ("state",):
+            d[name] = getattr(self, name).to_host_f32().copy()
+        return d
+
+    def _table(self, begin, end):
+        """Addresses, sizes and decays of the tensors in an arena range."""
+        md = self.model
+        states = (self.m.main_ptr, self.v.main_ptr) if self.state_bits == 32 else (self.state.main_ptr,)
+        key = (begin, end, md.params.main_ptr, md.grads.main_ptr, states, self.weight_decay)
+        if key not in self._tables:
+            if len(self._tables) > 64:
+                self._tables.clear()
+            on = (self._offs >= begin) & (self._offs < end)
+            o, four = self._offs[on], np.uint64(4)
+            at = [np.uint64(base) + o * four for base in (md.params.main_ptr, md.grads.main_ptr)]
+            unit = o * four if self.state_bits == 32 else o // np.uint64(64) * np.uint64(136)
+            at += [np.uint64(base) + unit for base in states]
+            self._tables[key] = (*at, self._n[on], np.where(self._matrix[on], np.float32(self.weight_decay), np.float32(0)))
+        return self._tables[key]
+
+    def _enqueue(self, begin=0, end=None, scalars=None):
+        table = self._table(begin, self.model.n_arena if end is None else end)
+        if not len(table[0]):
+            return
+        hyper = 0 if scalars is not None else self._hyper.main_ptr
+        if self.state_bits == 32:
+            sc.adamw_step(*table, *(scalars or [0.0] * 9), hyper=hyper)
+        else:
+            sc.adamw8_step(*table, *(scalars or [0.0] * 10), hyper=hyper, first=begin)

@@ -62,6 +62,8 @@ class Trainer:
         o = work.opt
         if o["kind"] == "adam":
             self.opt = S.Adam(self.model, lr=o["lr"], beta1=o.get("beta1", 0.9), beta2=o.get("beta2", 0.999), eps=o.get("eps", 1e-8))
+        elif o["kind"] == "adamw":
+            self.opt = S.AdamW(self.model, **{k: v for k, v in o.items() if k != "kind"})
         else:
             self.opt = S.SGD(self.model, lr=o["lr"], momentum=o.get("momentum", 0))
         L = S.Loss()

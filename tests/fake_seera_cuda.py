@@ -587,3 +587,113 @@ def unpool2_convT_act_bwd(w, x, y, g, dx, dw, db, N, Ci, H, W, act):
         cuda_unpooling_bwd(dup, dx, N, Ci, H, W, 2, 2)
     cuda_free(up)
     cuda_free(dup)
+
+
+# ---- layers over sequences and features, and AdamW: the 64-bit formulas, rounded once ------------------------------------------------
+def _columns(ptr, rows, C, ld):
+    """[rows, C] with rows `ld` floats apart, as a view."""
+    return np.lib.stride_tricks.as_strided(_view(ptr, (rows - 1) * ld + C), (rows, C), (4 * ld, 4))
+
+
+def gated_scan_fwd(f, v, ld, h0, lengths, h, last, N, T, C):
+    import sequence_np as ref
+    _count("gated_scan_fwd")
+    L = _view(lengths, N, np.int32) if lengths else None
+    H, S, _, _ = ref.scan_fwd(_columns(f, N * T, C, ld).reshape(N, T, C), _columns(v, N * T, C, ld).reshape(N, T, C), F(h0, (N, C)) if h0 else None, L)
+    if h:
+        F(h, (N, T, C))[:] = H
+    if last:
+        F(last, (N, C))[:] = S
+
+
+def gated_scan_bwd(f, v, ld, h0, lengths, h, dh, dlast, df, dv, ldg, dh0, N, T, C):
+    import sequence_np as ref
+    _count("gated_scan_bwd")
+    L = _view(lengths, N, np.int32) if lengths else None
+    opt = lambda p, s: F(p, s) if p else None  # noqa: E731
+    a, b, c, *_ = ref.scan_bwd(_columns(f, N * T, C, ld).reshape(N, T, C), _columns(v, N * T, C, ld).reshape(N, T, C), F(h, (N, T, C)),
+                               opt(dh, (N, T, C)), opt(dlast, (N, C)), opt(h0, (N, C)), L)
+    _columns(df, N * T, C, ldg)[:] = a.reshape(-1, C)
+    _columns(dv, N * T, C, ldg)[:] = b.reshape(-1, C)
+    if dh0:
+        F(dh0, (N, C))[:] = c
+
+
+_norm_eps = {}
+
+
+def norm_fwd(x, g, b, y, stats, rows, C, kind, eps):
+    import sequence_np as ref
+    _count("norm_fwd")
+    X = F(x, (rows, C))
+    F(y, (rows, C))[:] = ref.norm(X, _view(g, C), _view(b, C) if b else None, np.zeros_like(X), kind, eps)[0][0]
+    if stats:
+        _norm_eps[stats] = eps
+
+
+def norm_bwd(dy, x, g, stats, dx, dg, db, rows, C, kind):
+    import sequence_np as ref
+    _count("norm_bwd")
+    _, a, b, c = ref.norm(F(x, (rows, C)), _view(g, C), None, F(dy, (rows, C)), kind, _norm_eps[stats])
+    for p, w, s in ((dx, a, (rows, C)), (dg, b, (C,)), (db, c, (C,))):
+        if p:
+            F(p, s)[:] = w[0]
+
+
+def _residual(u, gate, ldg, res, ga, sc_, g2, b2, dout, dy, rows, C, kind, act, kind2, eps, eps2):
+    import sequence_np as ref
+    opt = lambda p, *s: F(p, s) if p else None  # noqa: E731
+    return ref.residual(F(u, (rows, C)), _columns(gate, rows, C, ldg) if gate else None, opt(res, rows, C), _view(ga, C), opt(sc_, C), opt(g2, C),
+                        opt(b2, C), opt(dout, rows, C), opt(dy, rows, C), kind, act, kind2, eps, eps2)
+
+
+def gated_residual_fwd(u, gate, ldg, res, ga, sc_, out, g2, b2, y, stats, rows, C, kind, act, kind2, eps, eps2):
+    _count("gated_residual_fwd")
+    fwd, _ = _residual(u, gate, ldg, res, ga, sc_, g2 if y else 0, b2, 0, 0, rows, C, kind, act, kind2, eps, eps2)
+    F(out, (rows, C))[:] = fwd[0][0]
+    if y:
+        F(y, (rows, C))[:] = fwd[1][0]
+    if stats:
+        _norm_eps[stats] = (eps, eps2)
+
+
+def gated_residual_bwd(dout, dy, u, gate, ldg, res, ga, sc_, g2, stats, du, dgate, lddg, dres, dga, dsc, dg2, db2, rows, C, kind, act, kind2):
+    _count("gated_residual_bwd")
+    _, b = _residual(u, gate, ldg, res, ga, sc_, g2 if dy else 0, 0, dout, dy, rows, C, kind, act, kind2, *_norm_eps[stats])
+    for p, k in ((du, "du"), (dres, "dres"), (dga, "dgamma"), (dsc, "dscale"), (dg2, "dgamma2"), (db2, "dbeta2")):
+        if p:
+            w = b[k][0]
+            F(p, w.shape)[:] = w
+    if dgate:
+        _columns(dgate, rows, C, lddg)[:] = b["dgate"][0]
+
+
+def grad_scale_update(g, n): _count("grad_scale_update")
+
+
+def _adamw_scalars(s, hyper, k): return [float(x) for x in _view(hyper, k)] if hyper else list(s)
+
+
+def adamw_step(w, g, m, v, n, decay, *s, hyper=0):
+    import sequence_np as ref
+    _count("adamw")
+    s = _adamw_scalars(s, hyper, 9)
+    for W, G, M, V, k, d in zip(*(np.asarray(a).tolist() for a in (w, g, m, v, n, decay))):
+        a, b, c, _ = ref.adamw(_view(W, k), _view(G, k), _view(M, k), _view(V, k), d, *s)
+        _view(W, k)[:], _view(M, k)[:], _view(V, k)[:] = a, b, c
+
+
+def adamw8_state_bytes(n): return -(-n // 64) * 136
+
+
+def adamw8_step(w, g, state, n, decay, *s, hyper=0, first=0):
+    import sequence_np as ref
+    _count("adamw8")
+    s = _adamw_scalars(s, hyper, 10)
+    for W, G, S, k, d in zip(*(np.asarray(a).tolist() for a in (w, g, state, n, decay))):
+        st = _view(S, adamw8_state_bytes(k), np.uint8)
+        m, v = ref.unpack8(st, k)
+        a, b, c, _ = ref.adamw(_view(W, k), _view(G, k), m, v, d, *s[:9])
+        _view(W, k)[:] = a
+        st[:] = ref.pack8(b, c, int(s[9]), first)
+        first += -(-k // 64) * 64
