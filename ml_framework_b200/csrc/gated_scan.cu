@@ -9,16 +9,22 @@
 //
 // Steps at and behind a sequence's length hold the state, write zeros and are not read.
 #include "common.cuh"
+#include "tc_ptx.cuh"
+#include <initializer_list>
 
 namespace seera {
 
+int *tc_status_word();                                    // contraction_tc.cu
+
 namespace {
+struct Waits { int *status; unsigned long long clocks; };  // where a wait that runs out is noted, and its budget
 struct ScanFwd {
     const float *f, *v, *h0;
     const int *lengths;
     float *h, *last;
     long long ld;
     int N, T, C, ranks;
+    Waits waits;
 };
 struct ScanBwd {
     const float *f, *v, *h0;
@@ -27,27 +33,31 @@ struct ScanBwd {
     float *df, *dv, *dh0;
     long long ld, ldg;
     int N, T, C, ranks;
+    Waits waits;
 };
 
 // A gate is kept as the smaller of a and 1 - a, which has its full relative precision, with the sign bit where that is a: a state that decays by
 // 1e-4 a step is summed over ten thousand of them, and one minus a rounded a would have lost four of seven digits there.
+// 1 / (1 + 2^t) with t = |f| log2 e; what t's rounding loses, up to |f| 2^-24 of the power, is made good by a factor of 1 + ln 2 times it (the
+// constant's own loses |f| 2^-26).  The two approximate instructions are off by at most 2^-22 and 2^-23: half the instructions that expf and a division
+// take, and instructions bound these kernels next to the bytes.  Beyond 88 the power would leave the range: s is 0 there, and below the smallest normal
+// number anyway.
 __device__ __forceinline__ float gate_of(float f) {
-    const float s = __fdividef(1.f, 1.f + expf(fabsf(f)));
-    return f > 0.f ? s : -s;
+    float x, e, s;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(fabsf(f)), "f"(88.f));
+    const float t = x * 1.44269502f, lost = fmaf(x, 1.44269502f, -t);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, lost * 0.693147182f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+    return copysignf(s, f);
 }
 constexpr float HOLD = 0.f;                               // the gate of a step that is not there: a = 1
 __device__ __forceinline__ bool keeps(float s) { return __float_as_int(s) >= 0; }       // (the sign of a zero counts)
-// a h + (1 - a) v
-__device__ __forceinline__ float step_of(float s, float h, float v) {
-    const bool k = keeps(s);
-    const float base = k ? h : v, to = k ? v : h;
-    return fmaf(fabsf(s), to - base, base);
-}
-// a x, and with (1 - a) x beside it
-__device__ __forceinline__ float decay(float s, float x) {
-    const float y = fabsf(s) * x;
-    return keeps(s) ? x - y : y;
-}
+// a h + (1 - a) v = h + s (v - h) or v - s (v - h)
+__device__ __forceinline__ float step_of(float s, float h, float v) { return fmaf(s, v - h, keeps(s) ? h : v); }
+// a x = x - s x or s x
+__device__ __forceinline__ float decay(float s, float x) { return fmaf(-s, x, keeps(s) ? x : 0.f); }
+// a x and (1 - a) x
 __device__ __forceinline__ void part(float s, float x, float &a_x, float &na_x) {
     const float y = fabsf(s) * x, z = x - y;
     a_x = keeps(s) ? z : y;
@@ -101,172 +111,421 @@ __global__ void __launch_bounds__(128) scan_bwd_serial_kernel(const __grid_const
     if (p.dh0) p.dh0[i] = s;
 }
 
-// ---- time split over warps and over the blocks of a cluster ---------------------------------------------------------------------------
-// A lane has one channel (a warp reads whole lines), a warp STEPS neighbouring steps of it in registers, a block WARPS of those and the blocks of a
-// cluster follow one another; the cluster then goes on to the next such piece of time, whose loads are on their way meanwhile.  What a run of steps
-// does to a state is one multiply-add, x -> A x + B: warps put theirs into shared memory, blocks send theirs to the others of the cluster, and
-// with the state at its start every warp goes over its registers again and writes.  One barrier of the block and one of the cluster a piece, with the
-// places in shared memory used in turn.
-constexpr int WARPS = 8, FWD_STEPS = 16, BWD_STEPS = 8, MAX_RANKS = 8;
+// ---- time split over half-warps, warps and the blocks of a cluster --------------------------------------------------------------------
+// A lane has two neighbouring channels of a tile of 32 (half a warp reads whole lines, and pairs halve what is not arithmetic), a half-warp L neighbouring
+// steps of them, a block W warps of those and the blocks of a cluster follow one another; the cluster then goes on to the next such piece of
+// time.  What a run of steps does to a state is one multiply-add, x -> A x + B.  A thread forms it for each of its steps from its first one on; warps put
+// theirs into shared memory, blocks send theirs to the others of the cluster; with the state at its start every step is one multiply-add more.
+// A warp copies its own steps into its own part of shared memory, STAGES - 1 pieces ahead: nothing waits for another warp's data, and the loads
+// cost neither registers nor, with 16 bytes a copy, more than a quarter of an instruction an element.  One barrier of the block a piece.
+// Between blocks the runs travel by stores that count their bytes on a barrier in the receiver's shared memory (a barrier of the cluster would wait for
+// every result written before it).  Two places are used in turn: who writes one for the second next piece has received everybody's run of the next
+// one, which each sends after all of its warps have read the place.
+// Measured (fp32, inputs beyond L2): forward of 8 x 2048 x 2048 76 us (5.3 TB/s, bytes bound it), of one sequence of 65536 x 512 108 us (3.7 TB/s;
+// with 13 blocks of 256 threads a tile the SMs wait for one another's runs and on shared memory, 36 % of the issue slots are used); backward of 8 x
+// 2048 x 2048 148 us (5.4 TB/s).  A lane with one channel and 16 steps took 80, 137 and 148 us, and a tile of 64 channels 102, 220 and 162.
+constexpr int MAX_RANKS = 16, STAGES = 3, TILE = 32, WARPS = 8, FWD_STEPS = 8, BWD_STEPS = 4;
 
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+struct __align__(8) Two { float x, y; };                  // a lane's two channels
+__device__ __forceinline__ unsigned long long bits(Two a) { return *reinterpret_cast<unsigned long long *>(&a); }
+__device__ __forceinline__ Two two(unsigned long long b) { return *reinterpret_cast<Two *>(&b); }
+__device__ __forceinline__ Two both(float x) { return Two{x, x}; }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return two(d);
 }
-__device__ __forceinline__ void send(float2 *mine, int rank, float2 v) {
-    unsigned local = (unsigned)__cvta_generic_to_shared(mine), remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+    return two(d);
 }
-__device__ __forceinline__ float2 then(float2 first, float2 second) { return make_float2(first.x * second.x, fmaf(second.x, first.y, second.y)); }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+    return two(d);
+}
+__device__ __forceinline__ Two less2(Two a, Two b) { return fma2(b, both(-1.f), a); }       // a - b
+__device__ __forceinline__ Two pick(bool kx, bool ky, Two a, Two b) { return Two{kx ? a.x : b.x, ky ? a.y : b.y}; }
+// gate_of for two, bit for bit
+__device__ __forceinline__ Two gate_of2(Two f) {
+    Two x, e, s;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x.x) : "f"(fabsf(f.x)), "f"(88.f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x.y) : "f"(fabsf(f.y)), "f"(88.f));
+    const Two t = mul2(x, both(1.44269502f)), gone = fma2(x, both(-1.44269502f), t);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = fma2(e, mul2(gone, both(-0.693147182f)), e);
+    e = add2(e, both(1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+    return Two{copysignf(s.x, f.x), copysignf(s.y, f.y)};
+}
 
-struct Joined {
-    float2 warps[2][WARPS][32], ranks[2][MAX_RANKS][32];
+struct __align__(16) Run { Two a, b; };                   // x -> a x + b for each of a lane's channels
+__device__ __forceinline__ Run no_steps() { return Run{both(1.f), both(0.f)}; }
+__device__ __forceinline__ Two after(const Run &r, Two x) { return fma2(r.a, x, r.b); }
+__device__ __forceinline__ Run then(const Run &first, const Run &second) { return Run{mul2(first.a, second.a), after(second, first.b)}; }
+template <int W> struct Joined {
+    Run warps[2][W][16], ranks[2][MAX_RANKS][16];
+    Two carry[2][16];
+    unsigned long long bar[2];
 };
-// The state at the start of this warp's steps, from that at the start of the piece; `carry` goes on to the start of the next one.
-__device__ __forceinline__ float join(Joined &sm, int buf, float2 mine, int warp, int lane, int rank, int ranks, float &carry) {
-    sm.warps[buf][warp][lane] = mine;
-    __syncthreads();
-    float2 before = make_float2(1.f, 0.f), all = before;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-        if (w == warp) before = all;
-        all = then(all, sm.warps[buf][w][lane]);
-    }
-    float x = carry;
-    if (ranks > 1) {
-        if (warp < ranks) send(&sm.ranks[buf][rank][lane], warp, all);        // a warp for each block of the cluster (at most WARPS of them)
-        cluster_sync();
-        for (int r = 0; r < ranks; r++) {
-            if (r == rank) x = carry;
-            const float2 o = sm.ranks[buf][r][lane];
-            carry = fmaf(o.x, carry, o.y);
-        }
-    } else {
-        carry = fmaf(all.x, carry, all.y);
-    }
-    return fmaf(before.x, x, before.y);
-}
 
-__global__ void __launch_bounds__(WARPS * 32, 2) scan_fwd_kernel(const __grid_constant__ ScanFwd p) {
-    constexpr int L = FWD_STEPS;
-    __shared__ Joined sm;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % p.ranks, tiles = (p.C + 31) / 32;
-    const unsigned tile = blockIdx.x / p.ranks;
-    const int n = tile / tiles, c = (tile - n * tiles) * 32 + lane;
-    const bool on = c < p.C;
-    const int len = on ? length_of(p.lengths, n, p.T) : 0;
-    const long long at = (long long)n * p.T;
-    const int piece = p.ranks * WARPS * L;
-    float carry = on && p.h0 ? p.h0[(long long)n * p.C + c] : 0.f;
-    float f[L], v[L];
-    auto request = [&](int t0) {
-        const float *pf = p.f + (at + t0) * p.ld + c, *pv = p.v + (at + t0) * p.ld + c;
-#pragma unroll
-        for (int i = 0; i < L; i++)
-            if (t0 + i < len) { f[i] = __ldcs(pf + i * p.ld); v[i] = __ldcs(pv + i * p.ld); }
-    };
-    int t0 = (rank * WARPS + warp) * L, buf = 0;
-    request(t0);
-    if (p.ranks > 1) cluster_sync();                        // the others' shared memory is there
-    for (int start = 0; start < p.T; start += piece, t0 += piece, buf ^= 1) {
-        float s[L], u[L];
-        float2 mine = make_float2(1.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < L; i++) {
-            s[i] = HOLD; u[i] = 0.f;
-            if (t0 + i < len) { s[i] = gate_of(f[i]); u[i] = v[i]; }
-            mine.y = step_of(s[i], mine.y, u[i]);
-            mine.x = decay(s[i], mine.x);
+__device__ __forceinline__ void send(Run *place, unsigned long long *bar, int rank, const Run &v) {
+    uint32_t to, done;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(place)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(done) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(v.a.x), "f"(v.a.y), "f"(v.b.x),
+                 "f"(v.b.y), "r"(done) : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded: a wait that runs out is noted, and the thread goes on without waiting any more (it still sends all it has to, and no block leaves early).
+__device__ __forceinline__ void await(uint32_t bar, uint32_t parity, Waits &w) {
+    if (arrived(bar, parity) || !w.clocks) return;
+    const long long t0 = clock64();
+    while (!arrived(bar, parity))
+        if ((unsigned long long)(clock64() - t0) > w.clocks) {
+            if (w.status) atomicCAS(w.status, 0, 5);
+            w.clocks = 0;
+            return;
         }
-        request(t0 + piece);
-        float x = join(sm, buf, mine, warp, lane, rank, p.ranks, carry);
-        if (p.h && on) {
-            float *h = p.h + (at + t0) * p.C + c;
+}
+// Copies of BYTES bytes from global into shared memory that the thread does not wait for.
+template <int BYTES> __device__ __forceinline__ void copy_async(float *to, const float *from) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+
+// Which channels, steps and sequence a thread has, and how its runs and those of others are joined.
+template <int W, int L> struct Place {
+    static constexpr int STEPS = 2 * L, ROWS = STEPS * TILE;        // of a warp, and the floats of a tensor that it copies of a piece
+    Joined<W> &sm;
+    int warp, lane, half, col, rank, ranks, n, c0, c, len, piece, first;
+    bool on, on2;                                          // whether the lane's channels are there
+    Waits waits;
+    Two carry;                                             // several blocks: the state at the start of the piece (one block has it in shared memory)
+    template <class P> __device__ __forceinline__ Place(const P &p, Joined<W> &sm_) : sm(sm_) {
+        warp = threadIdx.x >> 5; lane = threadIdx.x & 31; half = lane >> 4; col = lane & 15; ranks = p.ranks; rank = blockIdx.x % ranks;
+        const unsigned tiles = (p.C + TILE - 1) / TILE, tile = blockIdx.x / ranks;
+        n = tile / tiles;
+        c0 = (tile - n * tiles) * TILE;
+        c = c0 + 2 * col;
+        on = c < p.C; on2 = c + 1 < p.C;
+        len = length_of(p.lengths, n, p.T);
+        piece = ranks * W * STEPS;
+        first = (rank * W + warp) * STEPS;
+        waits = p.waits;
+    }
+    __device__ __forceinline__ Two state(const float *p, int C) const {
+        const long long i = (long long)n * C + c;
+        return Two{on && p ? p[i] : 0.f, on2 && p ? p[i + 1] : 0.f};
+    }
+    __device__ __forceinline__ void begin(Two x) {
+        carry = x;
+        if (ranks == 1) {
+            if (threadIdx.x < 16) sm.carry[0][col] = x;    // (read behind the first piece's barrier)
+            return;
+        }
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&sm.bar[0]), 1);
+            mbar_init(smem_u32(&sm.bar[1]), 1);
+            fence_mbar_init();
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // What the thread's steps of piece k do to a state (`run`) is given out.  Afterwards `run` is what the warp's other half does in front of it.
+    __device__ __forceinline__ void give(int k, Run &run) {
+        const int buf = k & 1;
+        Run other;
+        other.a = two(__shfl_xor_sync(0xffffffffu, bits(run.a), 16));
+        other.b = two(__shfl_xor_sync(0xffffffffu, bits(run.b), 16));
+        if (!half) sm.warps[buf][warp][col] = then(run, other);
+        run = half ? other : no_steps();
+        __syncthreads();
+        if (ranks > 1) {
+            Run all = sm.warps[buf][0][col];
+#pragma unroll
+            for (int i = 1; i < W; i++) all = then(all, sm.warps[buf][i][col]);
+            if (threadIdx.x == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&sm.bar[buf])), "r"(ranks * 16 * (int)sizeof(Run)) : "memory");
+            for (int r = 2 * warp + half; r < ranks; r += 2 * W) send(&sm.ranks[buf][rank][col], &sm.bar[buf], r, all);
+        }
+    }
+    // The state at the start of the thread's steps of piece k.
+    __device__ __forceinline__ Two receive(int k, const Run &before) {
+        const int buf = k & 1;
+        Two x;
+        if (ranks > 1) {
+            await(smem_u32(&sm.bar[buf]), (k >> 1) & 1, waits);
+            x = carry;
+#pragma unroll 4
+            for (int r = 0; r < rank; r++) x = after(sm.ranks[buf][r][col], x);
+            carry = x;
+#pragma unroll 4
+            for (int r = rank; r < ranks; r++) carry = after(sm.ranks[buf][r][col], carry);
+        } else {
+            x = sm.carry[buf][col];
+        }
+#pragma unroll
+        for (int i = 0; i < W - 1; i++)
+            if (i < warp) x = after(sm.warps[buf][i][col], x);
+        if (ranks == 1 && warp == W - 1 && !half) sm.carry[buf ^ 1][col] = after(sm.warps[buf][W - 1][col], x);
+        return after(before, x);
+    }
+    // The state behind the last of k pieces goes to `last`.  No block leaves while another may still send to it: every block has waited for all
+    // that is sent to it, which the cluster's barrier makes sure of where a wait has run out.
+    __device__ __forceinline__ void end(int k, float *last, int C) {
+        if (ranks == 1) __syncthreads();
+        if (last && rank == 0 && threadIdx.x < 16) {
+            if (ranks == 1) carry = sm.carry[k & 1][col];
+            const long long i = (long long)n * C + c;
+            if (on) last[i] = carry.x;
+            if (on2) last[i + 1] = carry.y;
+        }
+        if (ranks == 1) return;
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    }
+    // Steps t0 .. t0 + STEPS - 1 of a tensor whose rows are `ld` floats apart into to[STEPS][TILE], those of them in [lo, len); `from`: where row t0 of
+    // this sequence and channel 0 are.
+    template <int BYTES> __device__ __forceinline__ void copy(float *to, const float *from, int t0, long long ld, int lo, int C) const {
+        constexpr int PER = BYTES / 4, ACROSS = TILE / PER, DOWN = 32 / ACROSS;
+        const int x = lane % ACROSS * PER, y = lane / ACROSS;
+        if (c0 + x >= C) return;
+        const float *p = from + y * ld + c0 + x;
+        float *t = to + y * TILE + x;
+        if (t0 >= lo && t0 + STEPS <= len) {
+#pragma unroll
+            for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld) copy_async<BYTES>(t + i * TILE, p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld)
+                if (t0 + i + y >= lo && t0 + i + y < len) copy_async<BYTES>(t + i * TILE, p);
+        }
+    }
+    // The lane's channels to row `p` points to; pairs where PAIRS says that they lie on 8 bytes.
+    template <bool PAIRS> __device__ __forceinline__ void put(float *p, Two v) const {
+        if (PAIRS) {
+            __stcs(reinterpret_cast<float2 *>(p), make_float2(v.x, v.y));
+        } else {
+            __stcs(p, v.x);
+            if (on2) __stcs(p + 1, v.y);
+        }
+    }
+};
+
+template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 / W) scan_fwd_kernel(const __grid_constant__ ScanFwd p) {
+    typedef Place<W, L> Me;
+    constexpr int ROWS = Me::ROWS;
+    __shared__ Joined<W> sm;
+    extern __shared__ __align__(16) float stages[];         // [STAGES][W][f, v][2 L][TILE]
+    Me me(p, sm);
+    const long long at = (long long)me.n * p.T;
+    float *mine = stages + me.warp * 2 * ROWS;
+    auto request = [&](int t0, int stage) {
+        float *to = mine + stage * W * 2 * ROWS;
+        if (t0 < me.len) {
+            me.template copy<BYTES>(to, p.f + (at + t0) * p.ld, t0, p.ld, 0, p.C);
+            me.template copy<BYTES>(to + ROWS, p.v + (at + t0) * p.ld, t0, p.ld, 0, p.C);
+        }
+        copies_commit();
+    };
+    int t0 = me.first, stage = 0;
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; k++) request(t0 + k * me.piece, k);
+    me.begin(me.state(p.h0, p.C));
+    const int own = me.half * L;                            // the thread's steps among the warp's
+    auto work = [&](Run (&m)[L], int t0) {                  // the steps as one multiply-add each from the thread's first one on
+        copies_wait();
+        __syncwarp();                                       // the piece is there for every lane, and the stage before it is read
+        request(t0 + (STAGES - 1) * me.piece, stage == 0 ? STAGES - 1 : stage - 1);
+        const float *from = mine + stage * W * 2 * ROWS + own * TILE + 2 * me.col;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        auto steps = [&](bool all) {
+            Run run = no_steps();
 #pragma unroll
             for (int i = 0; i < L; i++) {
-                x = step_of(s[i], x, u[i]);
-                if (t0 + i < p.T) __stcs(h + (long long)i * p.C, t0 + i < len ? x : 0.f);
+                if (all || t0 + own + i < me.len) {
+                    const Two f = *reinterpret_cast<const Two *>(from + i * TILE), v = *reinterpret_cast<const Two *>(from + ROWS + i * TILE), s = gate_of2(f);
+                    const bool kx = keeps(s.x), ky = keeps(s.y);
+                    run.b = fma2(s, less2(v, run.b), pick(kx, ky, run.b, v));
+                    run.a = fma2(Two{-s.x, -s.y}, run.a, pick(kx, ky, run.a, both(0.f)));
+                }
+                m[i] = run;
             }
+        };
+        if (t0 + Me::STEPS <= me.len) steps(true);
+        else steps(false);
+    };
+    auto write = [&](const Run (&m)[L], Two x, int t0) {
+        t0 += own;
+        if (!p.h || !me.on || t0 >= p.T) return;
+        float *h = p.h + (at + t0) * p.C + me.c;
+        if (t0 + L <= me.len) {
+#pragma unroll
+            for (int i = 0; i < L; i++, h += p.C) me.template put<BYTES == 16>(h, after(m[i], x));
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; i++, h += p.C)
+                if (t0 + i < p.T) me.template put<BYTES == 16>(h, t0 + i < me.len ? after(m[i], x) : both(0.f));
         }
+    };
+    int k = 0;
+    auto go = [&](const Run (&now)[L], Run (&next)[L]) {    // `now` has been worked on
+        Run before = now[L - 1];
+        me.give(k, before);
+        work(next, t0 + me.piece);                          // (while the others' runs are on their way)
+        write(now, me.receive(k, before), t0);
+        t0 += me.piece;
+        k++;
+    };
+    Run one[L], two[L];
+    work(one, t0);
+    for (long long start = 0; start < p.T; start += 2 * me.piece) {
+        go(one, two);
+        if (start + me.piece >= p.T) break;
+        go(two, one);
     }
-    if (on && p.last && rank == 0 && warp == 0) p.last[(long long)n * p.C + c] = carry;
+    me.end(k, p.last, p.C);
 }
 
 // Backward: the same with time running from the end, where c -> a (dh + c) is what a step does.
-__global__ void __launch_bounds__(WARPS * 32, 2) scan_bwd_kernel(const __grid_constant__ ScanBwd p) {
-    constexpr int L = BWD_STEPS;
-    __shared__ Joined sm;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % p.ranks, tiles = (p.C + 31) / 32;
-    const unsigned tile = blockIdx.x / p.ranks;
-    const int n = tile / tiles, c = (tile - n * tiles) * 32 + lane;
-    const bool on = c < p.C;
-    const int len = on ? length_of(p.lengths, n, p.T) : 0;
-    const long long at = (long long)n * p.T, state = (long long)n * p.C + c;
-    const int piece = p.ranks * WARPS * L;
-    float carry = on && p.dlast ? p.dlast[state] : 0.f;
-    float f[L], v[L], d[L], b[L];
-    auto request = [&](int t1) {                            // steps t1, t1 - 1, ...
-#pragma unroll
-        for (int i = 0; i < L; i++) {
-            const int t = t1 - i;
-            if (t >= 0 && t < len) {
-                const long long row = at + t;
-                f[i] = __ldcs(p.f + row * p.ld + c);
-                v[i] = __ldcs(p.v + row * p.ld + c);
-                d[i] = p.dh ? __ldcs(p.dh + row * p.C + c) : 0.f;
-                b[i] = t ? __ldcs(p.h + (row - 1) * p.C + c) : (p.h0 ? p.h0[state] : 0.f);
-            }
+template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 / W) scan_bwd_kernel(const __grid_constant__ ScanBwd p) {
+    typedef Place<W, L> Me;
+    constexpr int ROWS = Me::ROWS;
+    __shared__ Joined<W> sm;
+    extern __shared__ __align__(16) float stages[];         // [STAGES][W][f, v, dh, h of the step before][2 L][TILE]
+    Me me(p, sm);
+    const long long at = (long long)me.n * p.T;
+    float *mine = stages + me.warp * 4 * ROWS;
+    auto request = [&](int t0, int stage) {                 // steps t0 .. t0 + 2 L - 1, of which some may lie before the first
+        float *to = mine + stage * W * 4 * ROWS;
+        if (t0 + Me::STEPS > 0 && t0 < me.len) {
+            me.template copy<BYTES>(to, p.f + (at + t0) * p.ld, t0, p.ld, 0, p.C);
+            me.template copy<BYTES>(to + ROWS, p.v + (at + t0) * p.ld, t0, p.ld, 0, p.C);
+            if (p.dh) me.template copy<BYTES>(to + 2 * ROWS, p.dh + (at + t0) * p.C, t0, p.C, 0, p.C);
+            me.template copy<BYTES>(to + 3 * ROWS, p.h + (at + t0 - 1) * p.C, t0, p.C, 1, p.C);
         }
+        copies_commit();
     };
-    int t1 = p.T - 1 - (rank * WARPS + warp) * L, buf = 0;
-    request(t1);
-    if (p.ranks > 1) cluster_sync();
-    for (int start = 0; start < p.T; start += piece, t1 -= piece, buf ^= 1) {
-        float s[L], e[L], w[L];
-        float2 mine = make_float2(1.f, 0.f);
+    int t0 = p.T - me.first - Me::STEPS, stage = 0, k = 0;
 #pragma unroll
-        for (int i = 0; i < L; i++) {
-            const int t = t1 - i;
-            s[i] = HOLD; e[i] = 0.f; w[i] = 0.f;
-            if (t >= 0 && t < len) { s[i] = gate_of(f[i]); e[i] = d[i]; w[i] = b[i] - v[i]; }
-            mine.y = decay(s[i], e[i] + mine.y);
-            mine.x = decay(s[i], mine.x);
-        }
-        request(t1 - piece);
-        float x = join(sm, buf, mine, warp, lane, rank, p.ranks, carry);
-        if (on) {
+    for (int k = 0; k < STAGES - 1; k++) request(t0 - k * me.piece, k);
+    me.begin(me.state(p.dlast, p.C));
+    const Two h0 = me.state(p.h0, p.C);
+    const int own = (1 - me.half) * L;                      // the first half-warp has the later steps
+    for (; k * (long long)me.piece < p.T; k++, t0 -= me.piece) {
+        copies_wait();
+        __syncwarp();
+        request(t0 - (STAGES - 1) * me.piece, stage == 0 ? STAGES - 1 : stage - 1);
+        const float *from = mine + stage * W * 4 * ROWS + own * TILE + 2 * me.col;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        Two s[L], e[L], w[L];                               // gate, dh, h[t-1] - v[t]
+        Run run = no_steps();
+        auto work = [&](bool all) {
 #pragma unroll
-            for (int i = 0; i < L; i++) {
-                const int t = t1 - i;
-                if (t < 0) break;
-                const float g = e[i] + x, small = fabsf(s[i]);
-                float dv;
-                part(s[i], g, x, dv);
-                const bool there = t < len;
-                __stcs(p.df + (at + t) * p.ldg + c, there ? (1.f - small) * (small * g) * w[i] : 0.f);
-                __stcs(p.dv + (at + t) * p.ldg + c, there ? dv : 0.f);
+            for (int i = L - 1; i >= 0; i--) {
+                const int t = t0 + own + i;
+                s[i] = both(HOLD); e[i] = both(0.f); w[i] = both(0.f);
+                if (all || (t >= 0 && t < me.len)) {
+                    const float *row = from + i * TILE;
+                    Two h = *reinterpret_cast<const Two *>(row + 3 * ROWS);
+                    if (!all && t == 0) h = h0;
+                    s[i] = gate_of2(*reinterpret_cast<const Two *>(row));
+                    w[i] = less2(h, *reinterpret_cast<const Two *>(row + ROWS));
+                    if (p.dh) e[i] = *reinterpret_cast<const Two *>(row + 2 * ROWS);
+                    const bool kx = keeps(s[i].x), ky = keeps(s[i].y);
+                    const Two g = add2(e[i], run.b), ns = Two{-s[i].x, -s[i].y};
+                    run.b = fma2(ns, g, pick(kx, ky, g, both(0.f)));
+                    run.a = fma2(ns, run.a, pick(kx, ky, run.a, both(0.f)));
+                }
             }
+        };
+        if (t0 > 0 && t0 + Me::STEPS <= me.len) work(true);
+        else work(false);
+        me.give(k, run);
+        Two x = me.receive(k, run);
+        const int t1 = t0 + own;
+        if (me.on && t1 + L > 0) {
+            float *pf = p.df + (at + t1 + L - 1) * p.ldg + me.c, *pv = p.dv + (at + t1 + L - 1) * p.ldg + me.c;
+            auto write = [&](bool all) {
+#pragma unroll
+                for (int i = L - 1; i >= 0; i--, pf -= p.ldg, pv -= p.ldg) {
+                    const int t = t1 + i;
+                    if (!all && t < 0) break;
+                    const Two as = Two{fabsf(s[i].x), fabsf(s[i].y)}, g = add2(e[i], x), y = mul2(as, g), z = less2(g, y);
+                    const bool kx = keeps(s[i].x), ky = keeps(s[i].y);
+                    x = pick(kx, ky, z, y);
+                    Two dv = pick(kx, ky, y, z), df = mul2(mul2(less2(both(1.f), as), y), w[i]);
+                    if (!all && t >= me.len) dv = df = both(0.f);
+                    me.template put<BYTES == 16>(pf, df);
+                    me.template put<BYTES == 16>(pv, dv);
+                }
+            };
+            if (t1 >= 0 && t1 + L <= me.len) write(true);
+            else write(false);
         }
     }
-    if (on && p.dh0 && rank == 0 && warp == 0) p.dh0[state] = carry;
+    me.end(k, p.dh0, p.C);
 }
 
-// Blocks of a cluster: as many as it takes to give every SM two blocks, and no more than there are steps for.
-int ranks_of(int N, int T, int C, int steps) {
-    const long long tiles = (long long)N * ((C + 31) / 32);
-    int k = 1;
-    while (k < MAX_RANKS && tiles * k < 2 * rt().sm_count && (long long)k * WARPS * steps < T) k *= 2;
-    return k;
-}
-template <class P> cudaError_t launch_clusters(void (*kernel)(P), const P &p, long long tiles) {
+// Clusters of each size that are resident at once (0: not asked yet), as the device's groups of SMs and the kernel's resources allow.
+struct Resident { int clusters[MAX_RANKS + 1]; };
+// Blocks of a cluster: every cluster works through its tile's pieces one after the other, and the clusters that are not resident at once follow in
+// further rounds; the fewest pieces in a row win, and of equal sizes the smallest.  One sequence of 65536 steps and 512 channels, 16 tiles: 13 blocks take
+// 111 us, 8 take 151, and 16, of which 14 clusters are resident, 145.
+template <int W, class P> int launch_scan(void (*kernel)(P), Resident &known, P p, int steps, int tensors, const char *name) {
+    const long long tiles = (long long)p.N * ((p.C + TILE - 1) / TILE);
+    const size_t smem = (size_t)STAGES * W * tensors * steps * TILE * sizeof(float);
+    if (int s = check_cuda(allow_smem((const void *)kernel, smem), name)) return s;
+    // (more than 8 is not promised on every device)
+    if (!known.clusters[1]) {
+        if (int s = check_cuda(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), name)) return s;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * p.ranks)); cfg.blockDim = dim3(WARPS * 32); cfg.stream = rt().stream;
     cudaLaunchAttribute attr[1];
+    cfg.blockDim = dim3(W * 32); cfg.dynamicSmemBytes = smem; cfg.stream = rt().stream; cfg.attrs = attr;
     attr[0].id = cudaLaunchAttributeClusterDimension;
+    long long least = 0;
+    for (int r = 1; r <= MAX_RANKS; r++) {
+        int &resident = known.clusters[r];
+        if (!resident) {
+            attr[0].val.clusterDim.x = (unsigned)r; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3((unsigned)r); cfg.numAttrs = 1;
+            int most = 0;
+            if (int s = check_cuda(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg), name)) return s;
+            resident = most > 0 ? most : -1;
+        }
+        if (resident < 0 || tiles * r > 0x7fffffffLL) continue;
+        const long long row = ((tiles + resident - 1) / resident) * ((p.T + (long long)r * W * steps - 1) / ((long long)r * W * steps));
+        if (!least || row < least) { least = row; p.ranks = r; }
+    }
+    if (!least) return fail(SEERA_E_LIMIT, "%s: no block fits", name);
+    p.waits = Waits{p.ranks > 1 ? tc_status_word() : nullptr, rt().tc_wait_clocks};
+    if (p.ranks > 1) rt().tc_used = true;
+    cfg.gridDim = dim3((unsigned)(tiles * p.ranks));
     attr[0].val.clusterDim.x = (unsigned)p.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = p.ranks > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    cfg.numAttrs = p.ranks > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess) return check_cuda(e, name);
+    SEERA_LAUNCH_CHECK(name);
+    return SEERA_OK;
+}
+bool on16(std::initializer_list<const void *> ps) {
+    for (const void *p : ps) if (!aligned16(p)) return false;
+    return true;
+}
+bool on8(std::initializer_list<const void *> ps) {
+    for (const void *p : ps) if ((uintptr_t)p & 7) return false;
+    return true;
 }
 // Few steps: a thread per state has nothing to split.
 constexpr int SERIAL_STEPS = 16;
@@ -284,12 +543,17 @@ int seera_gated_scan_fwd(const float *gate, const float *cand, int ld, const flo
     if (N < 0 || T < 0 || C < 1 || ld < C || (!h && !h_last) || (N > 0 && T > 0 && (!gate || !cand))) return fail(SEERA_E_ARG, "gated_scan_fwd: bad argument");
     if ((long long)N * C > 0x7fffffffLL || T > (1 << 30)) return fail(SEERA_E_LIMIT, "gated_scan_fwd: %lld states, %d steps", (long long)N * C, T);
     if (N == 0) return SEERA_OK;
-    const ScanFwd p{gate, cand, h0, lengths, h, h_last, ld, N, T, C, ranks_of(N, T, C, FWD_STEPS)};
+    const ScanFwd p{gate, cand, h0, lengths, h, h_last, ld, N, T, C, 1, {}};
     ProfBytes pb((8.0 + (h ? 4 : 0)) * N * T * C, "gated_scan_fwd");
-    if (T <= SERIAL_STEPS) scan_fwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
-    else launch_clusters(scan_fwd_kernel, p, (long long)N * ((C + 31) / 32));
-    SEERA_LAUNCH_CHECK("gated_scan_fwd");
-    return SEERA_OK;
+    if (T <= SERIAL_STEPS) {
+        scan_fwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
+        SEERA_LAUNCH_CHECK("gated_scan_fwd");
+        return SEERA_OK;
+    }
+    const bool wide = C % 4 == 0 && ld % 4 == 0 && on16({gate, cand}) && on8({h});
+    static Resident known[2];
+    if (wide) return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, 16>, known[1], p, 2 * FWD_STEPS, 2, "gated_scan_fwd");
+    return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, 4>, known[0], p, 2 * FWD_STEPS, 2, "gated_scan_fwd");
 }
 
 int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const float *h0, const int *lengths, const float *h, const float *dh,
@@ -299,12 +563,17 @@ int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const flo
         return fail(SEERA_E_ARG, "gated_scan_bwd: bad argument");
     if ((long long)N * C > 0x7fffffffLL || T > (1 << 30)) return fail(SEERA_E_LIMIT, "gated_scan_bwd: %lld states, %d steps", (long long)N * C, T);
     if (N == 0) return SEERA_OK;
-    const ScanBwd p{gate, cand, h0, lengths, h, dh, dh_last, dgate, dcand, dh0, ld, ld_grad, N, T, C, ranks_of(N, T, C, BWD_STEPS)};
+    const ScanBwd p{gate, cand, h0, lengths, h, dh, dh_last, dgate, dcand, dh0, ld, ld_grad, N, T, C, 1, {}};
     ProfBytes pb((20.0 + (dh ? 4 : 0)) * N * T * C, "gated_scan_bwd");
-    if (T <= SERIAL_STEPS) scan_bwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
-    else launch_clusters(scan_bwd_kernel, p, (long long)N * ((C + 31) / 32));
-    SEERA_LAUNCH_CHECK("gated_scan_bwd");
-    return SEERA_OK;
+    if (T <= SERIAL_STEPS) {
+        scan_bwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
+        SEERA_LAUNCH_CHECK("gated_scan_bwd");
+        return SEERA_OK;
+    }
+    const bool wide = C % 4 == 0 && ld % 4 == 0 && ld_grad % 2 == 0 && on16({gate, cand, h, dh}) && on8({dgate, dcand});
+    static Resident known[2];
+    if (wide) return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, 16>, known[1], p, 2 * BWD_STEPS, 4, "gated_scan_bwd");
+    return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, 4>, known[0], p, 2 * BWD_STEPS, 4, "gated_scan_bwd");
 }
 
 }  // extern "C"
