@@ -59,18 +59,24 @@ __device__ __forceinline__ int tensor_of(const AdamWTable &tab, unsigned block) 
     }
     return lo;
 }
-// Every operation rounded by itself: the codes of the 8-bit form follow from these bits, and both forms keep the same averages.
-__device__ __forceinline__ void adamw_one(float &w, float g, float &m, float &v, const AdamWArgs &a, float keep) {
+// What a step needs of the scalars: w = keep w - rate m / (root sqrt(v) + eps).
+struct Update { float keep, rate, root; };
+__device__ __forceinline__ Update update_of(const AdamWArgs &a, float decay) { return Update{1.f - a.lr * decay, a.lr / a.c1, 1.f / sqrtf(a.c2)}; }
+// Every operation on the averages rounded by itself: the codes of the 8-bit form follow from these bits, and both forms keep the same averages.  The
+// weight's step takes the approximate square root (2^-23) and division (2^-22): of the step, which is a small part of the weight.
+__device__ __forceinline__ void adamw_one(float &w, float g, float &m, float &v, const AdamWArgs &a, const Update &u) {
     g = __fmul_rn(g, a.gs);
     m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(a.omb1, g));
     v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(a.omb2, __fmul_rn(g, g)));
-    w = w * keep - (a.lr * (m / a.c1)) / (sqrtf(v / a.c2) + a.eps);
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    w = fmaf(w, u.keep, -__fdividef(u.rate * m, fmaf(r, u.root, a.eps)));
 }
 
 __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ AdamWTable tab, const __grid_constant__ AdamWArgs by_value) {
     const AdamWTensor &t = tab.t[tensor_of(tab, blockIdx.x)];
     const AdamWArgs a = adamw_args(tab, by_value, false);
-    const float keep = 1.f - a.lr * t.decay;
+    const Update u = update_of(a, t.decay);
     const long long at = (long long)(blockIdx.x - t.first) * CHUNK;
     const int n = (int)min((long long)CHUNK, t.n - at);
     float *w = t.w + at, *m = (float *)t.m + at, *v = t.v + at;
@@ -85,15 +91,15 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int i = threadIdx.x + k * THREADS;
-            adamw_one(ww[k].x, gg[k].x, mm[k].x, vv[k].x, a, keep); adamw_one(ww[k].y, gg[k].y, mm[k].y, vv[k].y, a, keep);
-            adamw_one(ww[k].z, gg[k].z, mm[k].z, vv[k].z, a, keep); adamw_one(ww[k].w, gg[k].w, mm[k].w, vv[k].w, a, keep);
+            adamw_one(ww[k].x, gg[k].x, mm[k].x, vv[k].x, a, u); adamw_one(ww[k].y, gg[k].y, mm[k].y, vv[k].y, a, u);
+            adamw_one(ww[k].z, gg[k].z, mm[k].z, vv[k].z, a, u); adamw_one(ww[k].w, gg[k].w, mm[k].w, vv[k].w, a, u);
             ((float4 *)w)[i] = ww[k]; ((float4 *)m)[i] = mm[k]; ((float4 *)v)[i] = vv[k];
         }
         return;
     }
     for (int i = threadIdx.x; i < n; i += THREADS) {
         float ww = w[i], mm = m[i], vv = v[i];
-        adamw_one(ww, g[i], mm, vv, a, keep);
+        adamw_one(ww, g[i], mm, vv, a, u);
         w[i] = ww; m[i] = mm; v[i] = vv;
     }
 }
@@ -102,8 +108,11 @@ constexpr int BLOCK_ENTRIES = 64, BLOCK_BYTES = 136;
 constexpr float M_UNIT = 0x1p-112f, V_UNIT = 0x1p-96f;       // 1.0 times these has the exponent fields 15 and 31: the largest codes
 constexpr unsigned M_TOP = 0x78, V_TOP = 0xF8;
 
-__device__ __forceinline__ unsigned random32(unsigned long long place, unsigned step) {
-    unsigned x = (unsigned)place ^ ((unsigned)(place >> 32) * 0x632BE5ABu) ^ (step * 0x9E3779B1u);
+// The hash of a place and a step, its first line apart: four neighbouring places from a multiple of four on differ in it by their last two bits.
+__device__ __forceinline__ unsigned random_seed(unsigned long long place, unsigned step) {
+    return (unsigned)place ^ ((unsigned)(place >> 32) * 0x632BE5ABu) ^ (step * 0x9E3779B1u);
+}
+__device__ __forceinline__ unsigned random32(unsigned x) {
     x = (x ^ (x >> 16)) * 0xA3D95F4Bu;
     x = (x ^ (x >> 15)) * 0x6C8E9D73u;
     return x ^ (x >> 16);
@@ -127,7 +136,7 @@ __device__ __forceinline__ float largest_of(unsigned bits, float &inv) {
 __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__ AdamWTable tab, const __grid_constant__ AdamWArgs by_value) {
     const AdamWTensor &t = tab.t[tensor_of(tab, blockIdx.x)];
     const AdamWArgs a = adamw_args(tab, by_value, true);
-    const float keep = 1.f - a.lr * t.decay;
+    const Update u = update_of(a, t.decay);
     const unsigned step = (unsigned)a.step;
     const long long at = (long long)(blockIdx.x - t.first) * CHUNK;
     const int n = (int)min((long long)CHUNK, t.n - at);
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__
         for (int j = 0; j < 4; j++) {
             m[j] = decode_m((code[k].x >> (8 * j)) & 255u, top[k].x);
             v[j] = decode_v((code[k].y >> (8 * j)) & 255u, top[k].y);
-            adamw_one(ww[k][j], gg[k][j], m[j], v[j], a, keep);
+            adamw_one(ww[k][j], gg[k][j], m[j], v[j], a, u);
             if (i + j >= n) m[j] = v[j] = 0.f;                // places behind the tensor's end
             am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);      // as bits: a NaN is larger than all else, and its block shows it
             av = max(av, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -182,10 +191,10 @@ __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__
         float im, iv;
         const float lm = largest_of(am, im), lv = largest_of(av, iv);
         uint2 c = make_uint2(0, 0);
-        const unsigned long long place = (unsigned long long)(t.place + at + i);
+        const unsigned seed = random_seed((unsigned long long)(t.place + at + i), step);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const unsigned r = random32(place + j, step);
+            const unsigned r = random32(seed ^ j);
             c.x |= (encode(fabsf(m[j]), im, M_UNIT, M_TOP, r & 0xffffu) | (m[j] < 0.f ? 128u : 0u)) << (8 * j);
             c.y |= encode(v[j], iv, V_UNIT, V_TOP, r >> 16) << (8 * j);
         }
@@ -225,7 +234,7 @@ __global__ void __launch_bounds__(256) adamw8_read_kernel(const char *__restrict
 int adamw(bool eight, int count, float *const *w, const float *const *g, void *const *m, float *const *v, const long long *n, const float *decay,
           const AdamWArgs &a, const float *hyper, long long first, const char *name) {
     SEERA_ENSURE();
-    if (count < 0 || (count > 0 && (!w || !g || !m || !n || !decay || (!eight && !v))) || first < 0) return fail(SEERA_E_ARG, "%s: bad argument", name);
+    if (count < 0 || (count > 0 && (!w || !g || !m || !n || !decay || (!eight && !v))) || first < 0 || first % BLOCK_ENTRIES) return fail(SEERA_E_ARG, "%s: bad argument", name);
     double total = 0;
     for (int i = 0; i < count; i++) {
         if (n[i] < 0 || (n[i] > 0 && (!w[i] || !g[i] || !m[i] || (!eight && !v[i])))) return fail(SEERA_E_ARG, "%s: bad argument for tensor %d", name, i);

@@ -9,6 +9,7 @@
 //
 // Steps at and behind a sequence's length hold the state, write zeros and are not read.
 #include "common.cuh"
+#include "sigmoid.cuh"
 #include "tc_ptx.cuh"
 #include <initializer_list>
 
@@ -36,21 +37,8 @@ struct ScanBwd {
     Waits waits;
 };
 
-// A gate is kept as the smaller of a and 1 - a, which has its full relative precision, with the sign bit where that is a: a state that decays by
+// A gate is kept as sigmoid_less gives it, the smaller of a and 1 - a, which has its full relative precision, with the sign bit where that is a: a state that decays by
 // 1e-4 a step is summed over ten thousand of them, and one minus a rounded a would have lost four of seven digits there.
-// 1 / (1 + 2^t) with t = |f| log2 e; what t's rounding loses, up to |f| 2^-24 of the power, is made good by a factor of 1 + ln 2 times it (the
-// constant's own loses |f| 2^-26).  The two approximate instructions are off by at most 2^-22 and 2^-23: half the instructions that expf and a division
-// take, and instructions bound these kernels next to the bytes.  Beyond 88 the power would leave the range: s is 0 there, and below the smallest normal
-// number anyway.
-__device__ __forceinline__ float gate_of(float f) {
-    float x, e, s;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(fabsf(f)), "f"(88.f));
-    const float t = x * 1.44269502f, lost = fmaf(x, 1.44269502f, -t);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    e = fmaf(e, lost * 0.693147182f, e);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
-    return copysignf(s, f);
-}
 constexpr float HOLD = 0.f;                               // the gate of a step that is not there: a = 1
 __device__ __forceinline__ bool keeps(float s) { return __float_as_int(s) >= 0; }       // (the sign of a zero counts)
 // a h + (1 - a) v = h + s (v - h) or v - s (v - h)
@@ -83,7 +71,7 @@ __global__ void __launch_bounds__(128) scan_fwd_serial_kernel(const __grid_const
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             if (t + k >= p.T) break;
-            if (t + k < len) s = step_of(gate_of(ff[k]), s, vv[k]);
+            if (t + k < len) s = step_of(sigmoid_less(ff[k]), s, vv[k]);
             if (h) h[(long long)(t + k) * p.C] = t + k < len ? s : 0.f;
         }
     }
@@ -100,7 +88,7 @@ __global__ void __launch_bounds__(128) scan_bwd_serial_kernel(const __grid_const
         const long long row = at + t;
         float df = 0.f, dv = 0.f;
         if (t < len) {
-            const float gate = gate_of(p.f[row * p.ld + c]), g = (p.dh ? p.dh[row * p.C + c] : 0.f) + s;
+            const float gate = sigmoid_less(p.f[row * p.ld + c]), g = (p.dh ? p.dh[row * p.C + c] : 0.f) + s;
             const float before = t ? p.h[(row - 1) * p.C + c] : (p.h0 ? p.h0[i] : 0.f);
             part(gate, g, s, dv);
             df = (1.f - fabsf(gate)) * (fabsf(gate) * g) * (before - p.v[row * p.ld + c]);
@@ -147,8 +135,8 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
 }
 __device__ __forceinline__ Two less2(Two a, Two b) { return fma2(b, both(-1.f), a); }       // a - b
 __device__ __forceinline__ Two pick(bool kx, bool ky, Two a, Two b) { return Two{kx ? a.x : b.x, ky ? a.y : b.y}; }
-// gate_of for two, bit for bit
-__device__ __forceinline__ Two gate_of2(Two f) {
+// sigmoid_less of two, bit for bit
+__device__ __forceinline__ Two sigmoid_less2(Two f) {
     Two x, e, s;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(x.x) : "f"(fabsf(f.x)), "f"(88.f));
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(x.y) : "f"(fabsf(f.y)), "f"(88.f));
@@ -354,7 +342,7 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
 #pragma unroll
             for (int i = 0; i < L; i++) {
                 if (all || t0 + own + i < me.len) {
-                    const Two f = *reinterpret_cast<const Two *>(from + i * TILE), v = *reinterpret_cast<const Two *>(from + ROWS + i * TILE), s = gate_of2(f);
+                    const Two f = *reinterpret_cast<const Two *>(from + i * TILE), v = *reinterpret_cast<const Two *>(from + ROWS + i * TILE), s = sigmoid_less2(f);
                     const bool kx = keeps(s.x), ky = keeps(s.y);
                     run.b = fma2(s, less2(v, run.b), pick(kx, ky, run.b, v));
                     run.a = fma2(Two{-s.x, -s.y}, run.a, pick(kx, ky, run.a, both(0.f)));
@@ -439,7 +427,7 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
                     const float *row = from + i * TILE;
                     Two h = *reinterpret_cast<const Two *>(row + 3 * ROWS);
                     if (!all && t == 0) h = h0;
-                    s[i] = gate_of2(*reinterpret_cast<const Two *>(row));
+                    s[i] = sigmoid_less2(*reinterpret_cast<const Two *>(row));
                     w[i] = less2(h, *reinterpret_cast<const Two *>(row + ROWS));
                     if (p.dh) e[i] = *reinterpret_cast<const Two *>(row + 2 * ROWS);
                     const bool kx = keeps(s[i].x), ky = keeps(s[i].y);

@@ -13,10 +13,17 @@
 // the second norm read it again: forward 20 bytes an element (u, gate, res; out, y), backward 32 (dout, dy, u, gate, res; du, dgate,
 // dres); out and its normalised values are formed anew in the backward from what it reads anyway.  Means and squares in two steps over the
 // registers (first the mean, then the differences to it), sums in fp32 by halves.
-// Sums over the rows: a thread always has the same columns, so it adds up its part in shared memory without a barrier; a block writes its
-// sums once, and a last launch adds the blocks' in a fixed order: the same bits on every run.
+// Sums over the rows: a thread always has the same columns, so it adds up its part in registers; a block writes its sums once, and a last launch adds
+// the blocks' in a fixed order: the same bits on every run.
+// The backward kernels and the plain norm run as many blocks as are resident, each with the next rows on their way while it works on one: what is left
+// to wait for are two sums over the block's threads a row.  Measured (fp32, inputs beyond L2): norm of 16384 x 1280 31 us forward and 44 backward (5.1
+// TB/s) with 7 for the sums over the blocks; residual of 16384 x 2048 117 us forward (5.7 TB/s) and 208 backward (5.1 TB/s).  Loads straight into
+// registers, two blocks an SM and sums in shared memory took 297 for the last.
 #include "common.cuh"
 #include "internal.h"
+#include "sigmoid.cuh"
+#include "tc_ptx.cuh"
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -34,72 +41,178 @@ template <int V> __device__ __forceinline__ void store(float *p, const Piece<V> 
 template <> __device__ __forceinline__ void store<4>(float *p, const Piece<4> &v) { *reinterpret_cast<float4 *>(p) = make_float4(v.x[0], v.x[1], v.x[2], v.x[3]); }
 template <> __device__ __forceinline__ void store<1>(float *p, const Piece<1> &v) { *p = v.x[0]; }
 
-// Both sums over the G threads of a row; `buf` alternates between two parts of the shared memory, so one barrier a call is enough.
-template <int G> __device__ __forceinline__ float2 row_sum(float2 v, float2 (*sm)[32], int &buf) {
+// Sums over the threads of a row, a warp or a block; `buf` alternates between two parts of the shared memory, so one barrier a call is enough.
+// (The places of the up to 16 warps are read independently of one another, several at once; what lies behind the last warp's is not used.)
+struct __align__(16) Sums { float2 v[2][16]; };
+template <int G> __device__ __forceinline__ float2 row_sum(float2 v, Sums &sm, int &buf) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
     if (G > 32) {
-        if ((threadIdx.x & 31) == 0) sm[buf][threadIdx.x >> 5] = v;
+        if ((threadIdx.x & 31) == 0) sm.v[buf][threadIdx.x >> 5] = v;
         __syncthreads();
-        v = sm[buf][0];
+        v = {0.f, 0.f};
 #pragma unroll
-        for (int i = 1; i < G / 32; i++) { const float2 o = sm[buf][i]; v.x += o.x; v.y += o.y; }
+        for (int i = 0; i < 16; i += 2)
+            if (i * 32 < G) {
+                const float4 o = *reinterpret_cast<const float4 *>(&sm.v[buf][i]);
+                const bool more = (i + 1) * 32 < G;
+                v.x += o.x + (more ? o.z : 0.f); v.y += o.y + (more ? o.w : 0.f);
+            }
         buf ^= 1;
     }
     return v;
 }
+template <int G> __device__ __forceinline__ float row_sum(float x, Sums &sm, int &buf) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (G > 32) {
+        float *place = &sm.v[buf][0].x;
+        if ((threadIdx.x & 31) == 0) place[threadIdx.x >> 5] = x;
+        __syncthreads();
+        x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            if (i * 32 < G) {
+                const float4 o = *reinterpret_cast<const float4 *>(place + i);
+                const int left = G / 32 - i;
+                x += (o.x + (left > 1 ? o.y : 0.f)) + ((left > 2 ? o.z : 0.f) + (left > 3 ? o.w : 0.f));
+            }
+        buf ^= 1;
+    }
+    return x;
+}
 
 // sigmoid(x) and 1 - sigmoid(x), both to full relative precision
 __device__ __forceinline__ void sigmoid2(float x, float &p, float &q) {
-    const float e = expf(-fabsf(x)), r = 1.f / (1.f + e);
-    p = x >= 0.f ? r : e * r;
-    q = x >= 0.f ? e * r : r;
-    if (x != x) p = q = x;
+    const float s = fabsf(sigmoid_less(x)), b = 1.f - s;
+    p = x >= 0.f ? b : s;
+    q = x >= 0.f ? s : b;
 }
-__device__ __forceinline__ float gate_value(float g, int act) {
-    float p, q;
+template <int K, int V, class Fn> __device__ __forceinline__ void each(Piece<V> (&g)[K], Fn fn) {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int j = 0; j < V; j++) fn(k, j, g[k].x[j]);
+}
+// g -> act(g)
+template <int K, int V> __device__ __forceinline__ void gate_values(Piece<V> (&g)[K], int act) {
     switch (act) {
-        case SEERA_ACT_NONE: return g;
-        case SEERA_ACT_RELU: return g > 0.f ? g : 0.f;
-        case SEERA_ACT_TANH: return tanhf(g);
-        default: sigmoid2(g, p, q); return act == SEERA_ACT_SIGMOID ? p : g * p;
+        case SEERA_ACT_NONE: return;
+        case SEERA_ACT_RELU: each<K, V>(g, [](int, int, float &x) { x = x > 0.f ? x : 0.f; }); return;
+        case SEERA_ACT_TANH: each<K, V>(g, [](int, int, float &x) { x = tanhf(x); }); return;
+        case SEERA_ACT_SIGMOID: each<K, V>(g, [](int, int, float &x) { float p, q; sigmoid2(x, p, q); x = p; }); return;
+        default: each<K, V>(g, [](int, int, float &x) { float p, q; sigmoid2(x, p, q); x *= p; });
     }
 }
-__device__ __forceinline__ float gate_slope(float g, int act, float &value) {
-    float p, q;
+// g -> act(g), with act'(g) beside it
+template <int K, int V> __device__ __forceinline__ void gate_slopes(Piece<V> (&g)[K], Piece<V> (&slope)[K], int act) {
     switch (act) {
-        case SEERA_ACT_NONE: value = g; return 1.f;
-        case SEERA_ACT_RELU: value = g > 0.f ? g : 0.f; return g > 0.f ? 1.f : 0.f;
-        case SEERA_ACT_TANH: value = tanhf(g); return 1.f - value * value;
-        default:
-            sigmoid2(g, p, q);
-            if (act == SEERA_ACT_SIGMOID) { value = p; return p * q; }
-            value = g * p;
-            return p * (1.f + g * q);
+        case SEERA_ACT_NONE: each<K, V>(g, [&](int k, int j, float &) { slope[k].x[j] = 1.f; }); return;
+        case SEERA_ACT_RELU: each<K, V>(g, [&](int k, int j, float &x) { slope[k].x[j] = x > 0.f ? 1.f : 0.f; x = x > 0.f ? x : 0.f; }); return;
+        case SEERA_ACT_TANH: each<K, V>(g, [&](int k, int j, float &x) { x = tanhf(x); slope[k].x[j] = 1.f - x * x; }); return;
+        case SEERA_ACT_SIGMOID: each<K, V>(g, [&](int k, int j, float &x) { float p, q; sigmoid2(x, p, q); slope[k].x[j] = p * q; x = p; }); return;
+        default: each<K, V>(g, [&](int k, int j, float &x) { float p, q; sigmoid2(x, p, q); slope[k].x[j] = p * (1.f + x * q); x *= p; });
     }
 }
 
+// The rows of N tensors on their way to the thread that works on them, STAGES - 1 rows ahead: each thread copies what it will read itself, so that
+// nothing has to be waited for but its own copies, and the loads hold no registers.  Rows of more than 8 floats a thread would not leave room for it.
+// (A place of its own for each thread, at constant distances, took 331 us where the copies of a warp side by side take 222.)
+// With three tensors, the forward of the residual, loads into registers by twice the blocks are faster (16384 x 2048: 117 against 133 us), with
+// one 70 against 55, with two 108 against 83, with five 245 against 222.
+template <int K, int V> constexpr bool AHEAD = K * V <= 8;
+template <int G, int K, int V, int N> struct Ahead {
+    static constexpr bool ON = AHEAD<K, V> && N != 3;
+    static constexpr int STAGES = N > 2 ? 2 : 3;
+    static constexpr int STAGE = N * K * V * G;
+    static constexpr size_t FLOATS = ON ? STAGES * STAGE : 0;          // of a row
+    float *mine, *asked;                                   // asked: the stage that is asked for next
+    int t, C;
+    Piece<V> now[ON ? 1 : N][ON ? 1 : K];
+    __device__ __forceinline__ Ahead(float *mem, int t_, int C_) : mine(mem + (G == 32 ? (threadIdx.x >> 5) * FLOATS : 0) + t_ * V), asked(mine), t(t_), C(C_) {}
+    __device__ __forceinline__ float *place(int i, int k) const { return asked + (i * K + k) * (G * V); }
+    // a row of tensor i (null: zeros) is asked for; `next()` behind the last of them
+    __device__ __forceinline__ void request(int i, const float *row) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int c = (t + k * G) * V;
+            if constexpr (ON) {
+                if (!row || c >= C) continue;
+                if (V == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(i, k))), "l"(row + c) : "memory");
+                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(place(i, k))), "l"(row + c) : "memory");
+            } else {
+                now[i][k] = {};
+                if (row && c < C) now[i][k] = load<V>(row + c);
+            }
+        }
+    }
+    __device__ __forceinline__ void next() {
+        if (!ON) return;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asked = asked + STAGE == mine + STAGES * STAGE ? mine : asked + STAGE;
+    }
+    // The row that was asked for STAGES - 1 calls of `next()` ago is there, in the stage that is asked for next.
+    __device__ __forceinline__ void wait() { if (ON) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+    __device__ __forceinline__ Piece<V> take(int i, int k, bool there) const {
+        if constexpr (ON) return there && (t + k * G) * V < C ? load<V>(place(i, k)) : Piece<V>{};
+        else return now[i][k];
+    }
+};
+
+// Sums over the rows for the thread's columns, in registers where a row is short enough, else in shared memory.
+template <int G, int K, int V> struct Sum {
+    static constexpr bool ON = AHEAD<K, V>;
+    Piece<V> r[ON ? K : 1];
+    float *mem;
+    __device__ __forceinline__ Sum(float *mem_, int t, int C) : mem(mem_) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int c = (t + k * G) * V;
+            if constexpr (ON) r[k] = {};
+            else if (c < C) store<V>(mem + c, Piece<V>{});
+        }
+    }
+    template <class Fn> __device__ __forceinline__ void add(int k, int c, Fn what) {
+        if constexpr (ON) {
+#pragma unroll
+            for (int j = 0; j < V; j++) r[k].x[j] += what(j);
+        } else {
+            Piece<V> s = load<V>(mem + c);
+#pragma unroll
+            for (int j = 0; j < V; j++) s.x[j] += what(j);
+            store<V>(mem + c, s);
+        }
+    }
+    __device__ __forceinline__ void keep(int t, int C) const {         // to shared memory
+        if constexpr (ON)
+            for (int k = 0; k < K; k++) {
+                const int c = (t + k * G) * V;
+                if (c < C) store<V>(mem + c, r[k]);
+            }
+    }
+};
+
 // Moments of a row that its threads hold.
-template <int G, int K, int V> __device__ __forceinline__ float2 moments(const Piece<V> (&x)[K], int C, int kind, float eps, int t, float2 (*sm)[32],
-                                                                        int &buf) {
+template <int G, int K, int V> __device__ __forceinline__ float2 moments(const Piece<V> (&x)[K], int C, int kind, float eps, int t, Sums &sm,
+                                                                           int &buf) {
     const float inv = 1.f / (float)C;
     float mu = 0.f;
     if (kind == SEERA_NORM_LAYER) {
-        float2 s = {0.f, 0.f};
+        float s = 0.f;
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
-            for (int j = 0; j < V; j++) s.x += x[k].x[j];      // (places behind the row hold zeros)
-        mu = row_sum<G>(s, sm, buf).x * inv;
+            for (int j = 0; j < V; j++) s += x[k].x[j];        // (places behind the row hold zeros)
+        mu = row_sum<G>(s, sm, buf) * inv;
     }
-    float2 s = {0.f, 0.f};
+    float s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; k++)
         if ((t + k * G) * V < C) {
 #pragma unroll
-            for (int j = 0; j < V; j++) { const float d = x[k].x[j] - mu; s.x += d * d; }
+            for (int j = 0; j < V; j++) { const float d = x[k].x[j] - mu; s += d * d; }
         }
-    return make_float2(mu, 1.f / sqrtf(row_sum<G>(s, sm, buf).x * inv + eps));
+    return make_float2(mu, 1.f / sqrtf(row_sum<G>(s, sm, buf) * inv + eps));
 }
 
 struct NormFwd {
@@ -108,19 +221,31 @@ struct NormFwd {
     int rows, C, kind;
     float eps;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 : G) norm_fwd_kernel(const __grid_constant__ NormFwd p) {
-    __shared__ float2 sm[2][32];
+// A block's threads, and its rows side by side.
+template <int G> constexpr int THREADS_OF = G == 32 ? 256 : G;
+template <int G> constexpr int ROWS_OF = G == 32 ? 8 : 1;
+
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 1024 / THREADS_OF<G>) norm_fwd_kernel(const __grid_constant__ NormFwd p) {
+    __shared__ Sums sm;
+    extern __shared__ __align__(16) float mem[];
+    typedef Ahead<G, K, V, 1> Rows;
     int buf = 0;
-    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, R = G == 32 ? 8 : 1;
-    for (int row = blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * R) {
+    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, side = G == 32 ? threadIdx.x >> 5 : 0, step = gridDim.x * ROWS_OF<G>;
+    Rows in(mem, t, p.C);
+    unsigned row = blockIdx.x * ROWS_OF<G> + side;      // (rows + 2 step passes 31 bits, not 32)
+    auto request = [&](unsigned row) {
+        if (row < p.rows) in.request(0, p.x + (long long)row * p.C);
+        in.next();
+    };
+    if (Rows::ON)
+        for (int k = 0; k < Rows::STAGES - 1; k++) request(row + k * step);
+    for (; row < p.rows; row += step) {
+        request(Rows::ON ? row + (Rows::STAGES - 1) * step : row);
+        in.wait();
         const long long at = (long long)row * p.C;
         Piece<V> x[K];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (t + k * G) * V;
-            if (c < p.C) x[k] = load<V>(p.x + at + c);
-            else x[k] = {};
-        }
+        for (int k = 0; k < K; k++) x[k] = in.take(0, k, true);
         const float2 ms = moments<G, K, V>(x, p.C, p.kind, p.eps, t, sm, buf);
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -141,47 +266,66 @@ template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 :
     }
 }
 
+// A block's sums over its rows from shared memory [rows side by side][sums][C] to its place in global memory.
+template <int G> __device__ __forceinline__ void write_sums(const float *acc, float *partial, int all) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < all; c += blockDim.x) {
+        float r = acc[c];
+        for (int i = 1; i < ROWS_OF<G>; i++) r += acc[(size_t)i * all + c];
+        partial[(size_t)blockIdx.x * all + c] = r;
+    }
+}
+
 struct NormBwd {
     const float *dy, *x, *gamma, *stats;
     float *dx, *partial;
     int rows, C, kind;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 : G) norm_bwd_kernel(const __grid_constant__ NormBwd p) {
-    __shared__ float2 sm[2][32];
-    extern __shared__ float acc[];                         // [rows side by side][dgamma, dbeta][C]
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 512 / THREADS_OF<G>) norm_bwd_kernel(const __grid_constant__ NormBwd p) {
+    __shared__ Sums sm;
+    extern __shared__ __align__(16) float mem[];           // rows on their way, then (or instead) [rows side by side][dgamma, dbeta][C]
+    typedef Ahead<G, K, V, 2> Rows;
     int buf = 0;
-    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, R = G == 32 ? 8 : 1, lane_row = G == 32 ? threadIdx.x >> 5 : 0;
-    float *mine = acc + (size_t)lane_row * 2 * p.C;
-    for (int k = 0; k < K; k++) {
-        const int c = (t + k * G) * V;
-        if (c < p.C) { store<V>(mine + c, Piece<V>{}); store<V>(mine + p.C + c, Piece<V>{}); }
-    }
+    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, side = G == 32 ? threadIdx.x >> 5 : 0, step = gridDim.x * ROWS_OF<G>;
+    float *acc = mem + (size_t)side * 2 * p.C;
+    Sum<G, K, V> sg(acc, t, p.C), sb(acc + p.C, t, p.C);
+    Rows in(mem, t, p.C);
+    unsigned row = blockIdx.x * ROWS_OF<G> + side;      // (rows + 2 step passes 31 bits, not 32)
+    auto request = [&](unsigned row) {
+        if (row < p.rows) {
+            in.request(0, p.x + (long long)row * p.C);
+            in.request(1, p.dy + (long long)row * p.C);
+        }
+        in.next();
+    };
+    if (Rows::ON)
+        for (int k = 0; k < Rows::STAGES - 1; k++) request(row + k * step);
     const float inv = 1.f / (float)p.C;
-    for (int row = blockIdx.x * R + lane_row; row < p.rows; row += gridDim.x * R) {
-        const long long at = (long long)row * p.C;
-        const float2 ms = *reinterpret_cast<const float2 *>(p.stats + 2ll * row);
+    auto stats = [&](unsigned row) { return row < p.rows ? *reinterpret_cast<const float2 *>(p.stats + 2ll * row) : float2{}; };
+    float2 ms_next = stats(row);
+    for (; row < p.rows; row += step) {
+        const float2 ms = ms_next;
+        ms_next = stats(row + step);
+        request(Rows::ON ? row + (Rows::STAGES - 1) * step : row);
+        in.wait();
         Piece<V> n[K], d[K];
         float2 s = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int c = (t + k * G) * V;
-            if (c < p.C) { n[k] = load<V>(p.x + at + c); d[k] = load<V>(p.dy + at + c); }
-        }
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (t + k * G) * V;
+            n[k] = in.take(0, k, true);
+            d[k] = in.take(1, k, true);
             if (c >= p.C) break;
             const Piece<V> g = load<V>(p.gamma + c);
-            Piece<V> sg = load<V>(mine + c), sb = load<V>(mine + p.C + c);
+#pragma unroll
+            for (int j = 0; j < V; j++) n[k].x[j] = (n[k].x[j] - ms.x) * ms.y;
+            sg.add(k, c, [&](int j) { return d[k].x[j] * n[k].x[j]; });
+            sb.add(k, c, [&](int j) { return d[k].x[j]; });
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                n[k].x[j] = (n[k].x[j] - ms.x) * ms.y;
-                sg.x[j] += d[k].x[j] * n[k].x[j];
-                sb.x[j] += d[k].x[j];
                 d[k].x[j] *= g.x[j];
                 s.x += d[k].x[j]; s.y += d[k].x[j] * n[k].x[j];
             }
-            store<V>(mine + c, sg); store<V>(mine + p.C + c, sb);
         }
         s = row_sum<G>(s, sm, buf);
         const float m0 = p.kind == SEERA_NORM_LAYER ? s.x * inv : 0.f, m1 = s.y * inv;
@@ -192,15 +336,12 @@ template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 :
             Piece<V> o;
 #pragma unroll
             for (int j = 0; j < V; j++) o.x[j] = ms.y * (d[k].x[j] - m0 - n[k].x[j] * m1);
-            store<V>(p.dx + at + c, o);
+            store<V>(p.dx + (long long)row * p.C + c, o);
         }
     }
-    __syncthreads();
-    for (int c = threadIdx.x; c < 2 * p.C; c += blockDim.x) {
-        float r = acc[c];
-        for (int i = 1; i < R; i++) r += acc[(size_t)i * 2 * p.C + c];
-        p.partial[(size_t)blockIdx.x * 2 * p.C + c] = r;
-    }
+    __syncthreads();                                       // (the places of the rows are read)
+    sg.keep(t, p.C); sb.keep(t, p.C);
+    write_sums<G>(mem, p.partial, 2 * p.C);
 }
 
 struct ResidualFwd {
@@ -210,34 +351,43 @@ struct ResidualFwd {
     int rows, C, kind, act, kind2;
     float eps, eps2;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 : G) residual_fwd_kernel(const __grid_constant__ ResidualFwd p) {
-    __shared__ float2 sm[2][32];
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, (AHEAD<K, V> ? 1024 : 512) / THREADS_OF<G>) residual_fwd_kernel(const __grid_constant__ ResidualFwd p) {
+    __shared__ Sums sm;
+    extern __shared__ __align__(16) float mem[];
+    typedef Ahead<G, K, V, 3> Rows;
     int buf = 0;
-    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, R = G == 32 ? 8 : 1;
-    for (int row = blockIdx.x * R + (G == 32 ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * R) {
+    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, side = G == 32 ? threadIdx.x >> 5 : 0, step = gridDim.x * ROWS_OF<G>;
+    Rows in(mem, t, p.C);
+    unsigned row = blockIdx.x * ROWS_OF<G> + side;      // (rows + 2 step passes 31 bits, not 32)
+    auto request = [&](unsigned row) {
+        if (row < p.rows) {
+            in.request(0, p.u + (long long)row * p.C);
+            in.request(1, p.gate ? p.gate + row * p.ld_gate : nullptr);
+            in.request(2, p.res ? p.res + (long long)row * p.C : nullptr);
+        }
+        in.next();
+    };
+    if (Rows::ON)
+        for (int k = 0; k < Rows::STAGES - 1; k++) request(row + k * step);
+    for (; row < p.rows; row += step) {
+        request(Rows::ON ? row + (Rows::STAGES - 1) * step : row);
+        in.wait();
         const long long at = (long long)row * p.C;
         Piece<V> x[K], q[K], r[K];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (t + k * G) * V;
-            x[k] = {};
-            if (c < p.C) {
-                x[k] = load<V>(p.u + at + c);
-                if (p.gate) q[k] = load<V>(p.gate + row * p.ld_gate + c);
-                if (p.res) r[k] = load<V>(p.res + at + c);
-            }
-        }
+        for (int k = 0; k < K; k++) { x[k] = in.take(0, k, true); q[k] = in.take(1, k, p.gate); r[k] = in.take(2, k, p.res); }
         const float2 ms = moments<G, K, V>(x, p.C, p.kind, p.eps, t, sm, buf);
+        if (p.gate) gate_values<K, V>(q, p.act);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int c = (t + k * G) * V;
             if (c >= p.C) break;
             const Piece<V> g = load<V>(p.gamma + c);
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                float o = (x[k].x[j] - ms.x) * ms.y * g.x[j];
-                if (p.gate) o *= gate_value(q[k].x[j], p.act);
-                x[k].x[j] = o;
+            for (int j = 0; j < V; j++) x[k].x[j] = (x[k].x[j] - ms.x) * ms.y * g.x[j];
+            if (p.gate) {
+#pragma unroll
+                for (int j = 0; j < V; j++) x[k].x[j] *= q[k].x[j];
             }
             if (p.res) {
                 const Piece<V> s = load<V>(p.scale + c);
@@ -279,63 +429,77 @@ struct ResidualBwd {
     long long ld_gate, ld_dgate;
     int rows, C, kind, act, kind2;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 : G) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
-    __shared__ float2 sm[2][32];
-    extern __shared__ float acc[];                         // [rows side by side][dgamma, dscale, dgamma2, dbeta2][C], the last two with dy
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 576 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
+    __shared__ Sums sm;
+    extern __shared__ __align__(16) float mem[];           // rows on their way, then (or instead) [rows side by side][dgamma, dscale, dgamma2, dbeta2][C],
+    typedef Ahead<G, K, V, 5> Rows;                        // the last two with dy
     int buf = 0;
-    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, R = G == 32 ? 8 : 1, lane_row = G == 32 ? threadIdx.x >> 5 : 0;
+    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, side = G == 32 ? threadIdx.x >> 5 : 0, step = gridDim.x * ROWS_OF<G>;
     const int sums = p.dy ? 4 : 2;
-    float *mine = acc + (size_t)lane_row * sums * p.C;
-    for (int k = 0; k < K; k++) {
-        const int c = (t + k * G) * V;
-        if (c < p.C) for (int s = 0; s < sums; s++) store<V>(mine + s * p.C + c, Piece<V>{});
-    }
-    const float inv = 1.f / (float)p.C;
-    for (int row = blockIdx.x * R + lane_row; row < p.rows; row += gridDim.x * R) {
-        const long long at = (long long)row * p.C;
-        const float4 st = *reinterpret_cast<const float4 *>(p.stats + 4ll * row);        // mu, s, mu2, s2
-        Piece<V> n[K], g[K], r[K], d[K], e[K];
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (t + k * G) * V;
-            d[k] = {};
-            if (c < p.C) {
-                n[k] = load<V>(p.u + at + c);
-                if (p.gate) g[k] = load<V>(p.gate + row * p.ld_gate + c);
-                if (p.res) r[k] = load<V>(p.res + at + c);
-                if (p.dout) d[k] = load<V>(p.dout + at + c);
-                if (p.dy) e[k] = load<V>(p.dy + at + c);
-            }
+    float *acc = mem + (size_t)side * sums * p.C;
+    Sum<G, K, V> sum_gamma(acc, t, p.C), sum_scale(acc + p.C, t, p.C), sum_gamma2(acc + (sums - 2) * p.C, t, p.C), sum_beta2(acc + (sums - 1) * p.C, t, p.C);
+    Rows in(mem, t, p.C);
+    unsigned row = blockIdx.x * ROWS_OF<G> + side;      // (rows + 2 step passes 31 bits, not 32)
+    auto request = [&](unsigned row) {
+        if (row < p.rows) {
+            const long long at = (long long)row * p.C;
+            in.request(0, p.u + at);
+            in.request(1, p.gate ? p.gate + row * p.ld_gate : nullptr);
+            in.request(2, p.res ? p.res + at : nullptr);
+            in.request(3, p.dout ? p.dout + at : nullptr);
+            in.request(4, p.dy ? p.dy + at : nullptr);
         }
+        in.next();
+    };
+    if (Rows::ON)
+        for (int k = 0; k < Rows::STAGES - 1; k++) request(row + k * step);
+    const float inv = 1.f / (float)p.C;
+    auto stats = [&](unsigned row) { return row < p.rows ? *reinterpret_cast<const float4 *>(p.stats + 4ll * row) : float4{}; };
+    float4 st_next = stats(row);
+    for (; row < p.rows; row += step) {
+        const float4 st = st_next;                         // mu, s, mu2, s2
+        st_next = stats(row + step);
+        request(Rows::ON ? row + (Rows::STAGES - 1) * step : row);
+        in.wait();
+        const long long at = (long long)row * p.C;
+        Piece<V> n[K], g[K], slope[Rows::ON ? K : 1], r[K], d[K];
         float2 s = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int c = (t + k * G) * V;
-            if (c >= p.C) break;
+            n[k] = in.take(0, k, true);
 #pragma unroll
             for (int j = 0; j < V; j++) n[k].x[j] = (n[k].x[j] - st.x) * st.y;
+            g[k] = in.take(1, k, p.gate);
+            r[k] = in.take(2, k, p.res);
+            d[k] = in.take(3, k, p.dout);
         }
+        // (a row of many floats a thread has no registers for values and slopes at once: they are formed where they are used)
+        if constexpr (Rows::ON) { if (p.gate) gate_slopes<K, V>(g, slope, p.act); }
         if (p.dy) {
-            Piece<V> n2[K];
+            Piece<V> n2[K], e[K];
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int c = (t + k * G) * V;
+                e[k] = in.take(4, k, true);
                 if (c >= p.C) break;
                 const Piece<V> ga = load<V>(p.gamma + c), g2 = load<V>(p.gamma2 + c);
-                Piece<V> sc = {}, sg = load<V>(mine + 2 * p.C + c), sb = load<V>(mine + 3 * p.C + c);
+                Piece<V> sc = {}, q[1] = {g[k]};
                 if (p.res) sc = load<V>(p.scale + c);
+                if (!Rows::ON && p.gate) gate_values<1, V>(q, p.act);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
                     float o = n[k].x[j] * ga.x[j];
-                    if (p.gate) o *= gate_value(g[k].x[j], p.act);
+                    if (p.gate) o *= q[0].x[j];
                     if (p.res) o += sc.x[j] * r[k].x[j];
                     n2[k].x[j] = (o - st.z) * st.w;
-                    sg.x[j] += e[k].x[j] * n2[k].x[j];
-                    sb.x[j] += e[k].x[j];
+                }
+                sum_gamma2.add(k, c, [&](int j) { return e[k].x[j] * n2[k].x[j]; });
+                sum_beta2.add(k, c, [&](int j) { return e[k].x[j]; });
+#pragma unroll
+                for (int j = 0; j < V; j++) {
                     e[k].x[j] *= g2.x[j];
                     s.x += e[k].x[j]; s.y += e[k].x[j] * n2[k].x[j];
                 }
-                store<V>(mine + 2 * p.C + c, sg); store<V>(mine + 3 * p.C + c, sb);
             }
             s = row_sum<G>(s, sm, buf);
             const float m0 = p.kind2 == SEERA_NORM_LAYER ? s.x * inv : 0.f, m1 = s.y * inv;
@@ -352,33 +516,30 @@ template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 :
             const int c = (t + k * G) * V;
             if (c >= p.C) break;
             const Piece<V> ga = load<V>(p.gamma + c);
-            Piece<V> sg = load<V>(mine + c);
             if (p.res) {
                 const Piece<V> sc = load<V>(p.scale + c);
-                Piece<V> ss = load<V>(mine + p.C + c), o;
+                Piece<V> o;
+                sum_scale.add(k, c, [&](int j) { return d[k].x[j] * r[k].x[j]; });
 #pragma unroll
-                for (int j = 0; j < V; j++) { ss.x[j] += d[k].x[j] * r[k].x[j]; o.x[j] = sc.x[j] * d[k].x[j]; }
-                store<V>(mine + p.C + c, ss);
+                for (int j = 0; j < V; j++) o.x[j] = sc.x[j] * d[k].x[j];
                 if (p.dres) store<V>(p.dres + at + c, o);
             }
             if (p.gate) {
-                Piece<V> o;
+                Piece<V> o, q[1] = {g[k]}, sl[1] = {slope[Rows::ON ? k : 0]};
+                if (!Rows::ON) gate_slopes<1, V>(q, sl, p.act);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    float q;
-                    const float slope = gate_slope(g[k].x[j], p.act, q);
-                    o.x[j] = d[k].x[j] * (ga.x[j] * n[k].x[j]) * slope;
-                    d[k].x[j] *= q;
+                    o.x[j] = d[k].x[j] * (ga.x[j] * n[k].x[j]) * sl[0].x[j];
+                    d[k].x[j] *= q[0].x[j];
                 }
                 if (p.dgate) store<V>(p.dgate + row * p.ld_dgate + c, o);
             }
+            sum_gamma.add(k, c, [&](int j) { return d[k].x[j] * n[k].x[j]; });
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                sg.x[j] += d[k].x[j] * n[k].x[j];
                 d[k].x[j] *= ga.x[j];
                 s.x += d[k].x[j]; s.y += d[k].x[j] * n[k].x[j];
             }
-            store<V>(mine + c, sg);
         }
         s = row_sum<G>(s, sm, buf);
         const float m0 = p.kind == SEERA_NORM_LAYER ? s.x * inv : 0.f, m1 = s.y * inv;
@@ -392,13 +553,10 @@ template <int G, int K, int V> __global__ void __launch_bounds__(G == 32 ? 256 :
             store<V>(p.du + at + c, o);
         }
     }
-    __syncthreads();
-    const int all = sums * p.C;
-    for (int c = threadIdx.x; c < all; c += blockDim.x) {
-        float r = acc[c];
-        for (int i = 1; i < R; i++) r += acc[(size_t)i * all + c];
-        p.partial[(size_t)blockIdx.x * all + c] = r;
-    }
+    __syncthreads();                                       // (the places of the rows are read)
+    sum_gamma.keep(t, p.C); sum_scale.keep(t, p.C);
+    if (p.dy) { sum_gamma2.keep(t, p.C); sum_beta2.keep(t, p.C); }
+    write_sums<G>(mem, p.partial, sums * p.C);
 }
 
 // The blocks' sums added up in a fixed order, each of the up to four results to a place of its own (null: not wanted).
@@ -432,31 +590,26 @@ int param_sums(const float *partial, const ParamSums &to, int C, int sums, int b
 }
 
 template <int I> using Int = std::integral_constant<int, I>;
-// The threads of a row: the fewest that hold it in at most 16 floats of each tensor.
+// The threads of a row: the fewest of these that hold it in 8 floats of each tensor, or 512 with 16.
+template <class Fn, class K, class V> int by_threads(int C, Fn fn, K k, V v) {
+    if (C <= 256) return fn(Int<32>{}, k, v);
+    if (C <= 512) return fn(Int<64>{}, k, v);
+    if (C <= 1024) return fn(Int<128>{}, k, v);
+    if (C <= 1280) return fn(Int<160>{}, k, v);
+    if (C <= 1536) return fn(Int<192>{}, k, v);
+    if (C <= 2048) return fn(Int<256>{}, k, v);
+    return fn(Int<512>{}, k, v);
+}
 template <class Fn> int by_width(int C, bool vec, Fn fn) {
-    if (vec) {
-        if (C <= 128) return fn(Int<32>{}, Int<1>{}, Int<4>{});
-        if (C <= 256) return fn(Int<32>{}, Int<2>{}, Int<4>{});
-        if (C <= 512) return fn(Int<128>{}, Int<1>{}, Int<4>{});
-        if (C <= 1024) return fn(Int<128>{}, Int<2>{}, Int<4>{});
-        if (C <= 2048) return fn(Int<256>{}, Int<2>{}, Int<4>{});
-        if (C <= 4096) return fn(Int<512>{}, Int<2>{}, Int<4>{});
-        return fn(Int<512>{}, Int<4>{}, Int<4>{});
-    }
-    if (C <= 128) return fn(Int<32>{}, Int<4>{}, Int<1>{});
-    if (C <= 256) return fn(Int<32>{}, Int<8>{}, Int<1>{});
-    if (C <= 512) return fn(Int<128>{}, Int<4>{}, Int<1>{});
-    if (C <= 1024) return fn(Int<128>{}, Int<8>{}, Int<1>{});
-    if (C <= 2048) return fn(Int<256>{}, Int<8>{}, Int<1>{});
-    if (C <= 4096) return fn(Int<512>{}, Int<8>{}, Int<1>{});
-    return fn(Int<512>{}, Int<16>{}, Int<1>{});
+    if (C > 4096) return vec ? fn(Int<512>{}, Int<4>{}, Int<4>{}) : fn(Int<512>{}, Int<16>{}, Int<1>{});
+    return vec ? by_threads(C, fn, Int<2>{}, Int<4>{}) : by_threads(C, fn, Int<8>{}, Int<1>{});
 }
 // Blocks of a launch that keeps sums over the rows: as many as are resident at once, so that each writes its sums once.
 int resident_grid(const void *kernel, int threads, size_t smem, int rows, int rows_at_once, int *grid) {
     int per_sm = 0;
     if (int s = check_cuda(allow_smem(kernel, smem), "norm: shared memory")) return s;
     if (int s = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem), "norm: occupancy")) return s;
-    const long long need = (rows + rows_at_once - 1) / rows_at_once, most = (long long)rt().sm_count * (per_sm > 0 ? per_sm : 1);
+    const long long need = ((long long)rows + rows_at_once - 1) / rows_at_once, most = (long long)rt().sm_count * (per_sm > 0 ? per_sm : 1);
     *grid = (int)(need < most ? need : most);
     return SEERA_OK;
 }
@@ -483,7 +636,10 @@ int seera_norm_fwd(const float *x, const float *gamma, const float *beta, float 
     ProfBytes pb(8.0 * rows * C, "norm_fwd");
     return by_width(C, C % 4 == 0 && all16({x, gamma, beta, y}), [&](auto g_, auto k_, auto v_) {
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
-        norm_fwd_kernel<G, K, V><<<G == 32 ? (rows + 7) / 8 : rows, G == 32 ? 256 : G, 0, rt().stream>>>(p);
+        const size_t smem = ROWS_OF<G> * Ahead<G, K, V, 1>::FLOATS * sizeof(float);
+        int grid = (int)(((long long)rows + ROWS_OF<G> - 1) / ROWS_OF<G>);
+        if (Ahead<G, K, V, 1>::ON) if (int s = resident_grid((const void *)norm_fwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
+        norm_fwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("norm_fwd");
         return (int)SEERA_OK;
     });
@@ -498,14 +654,13 @@ int seera_norm_bwd(const float *dy, const float *x, const float *gamma, const fl
     ProfBytes pb(12.0 * rows * C, "norm_bwd");
     return by_width(C, C % 4 == 0 && all16({dy, x, gamma, dx}), [&](auto g_, auto k_, auto v_) {
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
-        const int R = G == 32 ? 8 : 1, threads = G == 32 ? 256 : G;
-        const size_t smem = (size_t)R * 2 * C * sizeof(float);
+        const size_t smem = ROWS_OF<G> * std::max(Ahead<G, K, V, 2>::FLOATS, (size_t)2 * C) * sizeof(float);
         int grid;
-        if (int s = resident_grid((const void *)norm_bwd_kernel<G, K, V>, threads, smem, rows, R, &grid)) return s;
+        if (int s = resident_grid((const void *)norm_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
         float *partial = (float *)scratch_alloc((size_t)grid * 2 * C * sizeof(float));
         if (!partial) return (int)SEERA_E_OOM;
         const NormBwd p{dy, x, gamma, stats, dx, partial, rows, C, kind};
-        norm_bwd_kernel<G, K, V><<<grid, threads, smem, rt().stream>>>(p);
+        norm_bwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
         count_launch();
         int s = check_cuda(cudaGetLastError(), "norm_bwd");
         if (!s) s = param_sums(partial, {{dgamma, dbeta, nullptr, nullptr}}, C, 2, grid, "norm_bwd(sums)");
@@ -529,7 +684,10 @@ int seera_gated_residual_fwd(const float *u, const float *gate, int ld_gate, con
     const bool vec = C % 4 == 0 && (!gate || ld_gate % 4 == 0) && all16({u, gate, res, gamma, res ? scale : nullptr, out, y, y ? next_gamma : nullptr, y ? next_beta : nullptr});
     return by_width(C, vec, [&](auto g_, auto k_, auto v_) {
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
-        residual_fwd_kernel<G, K, V><<<G == 32 ? (rows + 7) / 8 : rows, G == 32 ? 256 : G, 0, rt().stream>>>(p);
+        const size_t smem = ROWS_OF<G> * Ahead<G, K, V, 3>::FLOATS * sizeof(float);
+        int grid = (int)(((long long)rows + ROWS_OF<G> - 1) / ROWS_OF<G>);
+        if (Ahead<G, K, V, 3>::ON) if (int s = resident_grid((const void *)residual_fwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
+        residual_fwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("gated_residual_fwd");
         return (int)SEERA_OK;
     });
@@ -552,14 +710,13 @@ int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u,
     const int sums = dy ? 4 : 2;
     return by_width(C, vec, [&](auto g_, auto k_, auto v_) {
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
-        const int R = G == 32 ? 8 : 1, threads = G == 32 ? 256 : G;
-        const size_t smem = (size_t)R * sums * C * sizeof(float);
+        const size_t smem = ROWS_OF<G> * std::max(Ahead<G, K, V, 5>::FLOATS, (size_t)sums * C) * sizeof(float);
         int grid;
-        if (int s = resident_grid((const void *)residual_bwd_kernel<G, K, V>, threads, smem, rows, R, &grid)) return s;
+        if (int s = resident_grid((const void *)residual_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
         float *partial = (float *)scratch_alloc((size_t)grid * sums * C * sizeof(float));
         if (!partial) return (int)SEERA_E_OOM;
         const ResidualBwd p{dout, dy, u, gate, res, gamma, scale, next_gamma, stats, du, dgate, dres, partial, ld_gate, ld_dgate, rows, C, kind, act, next_kind};
-        residual_bwd_kernel<G, K, V><<<grid, threads, smem, rt().stream>>>(p);
+        residual_bwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
         count_launch();
         int s = check_cuda(cudaGetLastError(), "gated_residual_bwd");
         if (!s) s = param_sums(partial, {{dgamma, dscale, dnext_gamma, dnext_beta}}, C, sums, grid, "gated_residual_bwd(sums)");
