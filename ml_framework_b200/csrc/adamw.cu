@@ -7,7 +7,8 @@
 // A chunk belongs to one tensor, so that a tensor's decay is the block's.
 //
 // What bounds it: the bytes.  32 bits: w, m, v read and written and the gradient read, 28 bytes an entry.  8 bits: 12 for w and the gradient
-// and 2 x 136 / 64 for the averages.
+// and 2 x 136 / 64 for the averages; of 67 million entries 180 us, 6.1 TB/s (and 102 us to read them out, 6.7), when an entry takes 40 instructions.
+// With four entries a thread, one at a time and with exact roots and divisions it took 107 instructions and 300 us: the instructions bounded it.
 //
 // Averages in 8 bits.  64 neighbouring entries of a tensor share a block of 136 bytes: sixteen times four codes of m and four of v (what a
 // thread reads and writes, in one piece), then the largest |m| and the largest v as floats.  A code is an entry over the block's largest, as a
@@ -19,6 +20,8 @@
 // entry's place and the step, so a step is reproducible.  The weights are updated from the averages as they are before rounding.
 #include "common.cuh"
 #include "internal.h"
+#include "pairs.cuh"
+#include <cuda_fp16.h>
 #include <memory>
 #include <string.h>
 
@@ -34,10 +37,10 @@ struct AdamWTensor {
     void *m;                                  // 8 bits: the blocks of both averages
     union { float *v; long long place; };     // 8 bits: number of the tensor's first entry, for the random bits
     long long n;
-    float decay;
-    unsigned first;                           // first block of the launch that works on it
 };
 struct AdamWTable {
+    unsigned first[TABLE];                    // of each tensor's blocks; side by side, so that the search waits for few lines of the arguments
+    float decay[TABLE];
     AdamWTensor t[TABLE];
     const float *hyper;                       // where not null, the scalars are there
     int count;
@@ -54,46 +57,72 @@ __device__ __forceinline__ int tensor_of(const AdamWTable &tab, unsigned block) 
     int lo = 0, hi = tab.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (tab.t[mid].first <= block) lo = mid;
+        if (tab.first[mid] <= block) lo = mid;
         else hi = mid - 1;
     }
     return lo;
 }
-// What a step needs of the scalars: w = keep w - rate m / (root sqrt(v) + eps).
+// What a step needs of the scalars: w = keep w + rate m / (root sqrt(v) + eps).
 struct Update { float keep, rate, root; };
-__device__ __forceinline__ Update update_of(const AdamWArgs &a, float decay) { return Update{1.f - a.lr * decay, a.lr / a.c1, 1.f / sqrtf(a.c2)}; }
-// Every operation on the averages rounded by itself: the codes of the 8-bit form follow from these bits, and both forms keep the same averages.  The
-// weight's step takes the approximate square root (2^-23) and division (2^-22): of the step, which is a small part of the weight.
-__device__ __forceinline__ void adamw_one(float &w, float g, float &m, float &v, const AdamWArgs &a, const Update &u) {
-    g = __fmul_rn(g, a.gs);
-    m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(a.omb1, g));
-    v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(a.omb2, __fmul_rn(g, g)));
+__device__ __forceinline__ Update update_of(const AdamWArgs &a, float decay) { return Update{1.f - a.lr * decay, -a.lr / a.c1, 1.f / sqrtf(a.c2)}; }
+__device__ __forceinline__ float largest(float a, float b) {            // a NaN wins
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-    w = fmaf(w, u.keep, -__fdividef(u.rate * m, fmaf(r, u.root, a.eps)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
+// The approximate square root is off by 2^-23; what lies below the smallest normal number counts as that (the flush would make it zero).
+__device__ __forceinline__ float root_of(float v) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(largest(v, 1.17549435e-38f)));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// (A sum of two at once would be contracted with the products before it.)
+__device__ __forceinline__ Two sum_of(Two a, Two b) { return Two{__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
+// Two entries.  Every operation on the averages rounded by itself: the codes of the 8-bit form follow from these bits, and both forms keep the same
+// averages.  The weight's step takes the approximate root and reciprocal (2^-23 each): of the step, which is a small part of the weight.
+__device__ __forceinline__ void adamw_two(Two &w, Two g, Two &m, Two &v, const AdamWArgs &a, const Update &u) {
+    g = mul2(g, both(a.gs));
+    m = sum_of(mul2(both(a.b1), m), mul2(both(a.omb1), g));
+    v = sum_of(mul2(both(a.b2), v), mul2(both(a.omb2), mul2(g, g)));
+    const Two d = fma2(Two{root_of(v.x), root_of(v.y)}, both(u.root), both(a.eps));
+    w = fma2(w, both(u.keep), mul2(mul2(both(u.rate), m), Two{reciprocal(d.x), reciprocal(d.y)}));
+}
+__device__ __forceinline__ void adamw_one(float &w, float g, float &m, float &v, const AdamWArgs &a, const Update &u) {
+    Two ww = both(w), mm = both(m), vv = both(v);
+    adamw_two(ww, both(g), mm, vv, a, u);
+    w = ww.x; m = mm.x; v = vv.x;
+}
+struct __align__(16) Four { Two lo, hi; };
 
 __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ AdamWTable tab, const __grid_constant__ AdamWArgs by_value) {
-    const AdamWTensor &t = tab.t[tensor_of(tab, blockIdx.x)];
+    const int number = tensor_of(tab, blockIdx.x);
+    const AdamWTensor &t = tab.t[number];
     const AdamWArgs a = adamw_args(tab, by_value, false);
-    const Update u = update_of(a, t.decay);
-    const long long at = (long long)(blockIdx.x - t.first) * CHUNK;
+    const Update u = update_of(a, tab.decay[number]);
+    const long long at = (long long)(blockIdx.x - tab.first[number]) * CHUNK;
     const int n = (int)min((long long)CHUNK, t.n - at);
     float *w = t.w + at, *m = (float *)t.m + at, *v = t.v + at;
     const float *g = t.g + at;
     if (n == CHUNK && !(((uintptr_t)w | (uintptr_t)m | (uintptr_t)v | (uintptr_t)g) & 15)) {
-        float4 ww[2], gg[2], mm[2], vv[2];
+        Four ww[2], gg[2], mm[2], vv[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int i = threadIdx.x + k * THREADS;
-            ww[k] = ((float4 *)w)[i]; gg[k] = __ldcs((const float4 *)g + i); mm[k] = ((float4 *)m)[i]; vv[k] = ((float4 *)v)[i];
+            ww[k] = ((Four *)w)[i]; mm[k] = ((Four *)m)[i]; vv[k] = ((Four *)v)[i];
+            const float4 x = __ldcs((const float4 *)g + i);
+            gg[k] = Four{{x.x, x.y}, {x.z, x.w}};
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int i = threadIdx.x + k * THREADS;
-            adamw_one(ww[k].x, gg[k].x, mm[k].x, vv[k].x, a, u); adamw_one(ww[k].y, gg[k].y, mm[k].y, vv[k].y, a, u);
-            adamw_one(ww[k].z, gg[k].z, mm[k].z, vv[k].z, a, u); adamw_one(ww[k].w, gg[k].w, mm[k].w, vv[k].w, a, u);
-            ((float4 *)w)[i] = ww[k]; ((float4 *)m)[i] = mm[k]; ((float4 *)v)[i] = vv[k];
+            adamw_two(ww[k].lo, gg[k].lo, mm[k].lo, vv[k].lo, a, u);
+            adamw_two(ww[k].hi, gg[k].hi, mm[k].hi, vv[k].hi, a, u);
+            ((Four *)w)[i] = ww[k]; ((Four *)m)[i] = mm[k]; ((Four *)v)[i] = vv[k];
         }
         return;
     }
@@ -106,9 +135,8 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const __grid_constant__ 
 
 constexpr int BLOCK_ENTRIES = 64, BLOCK_BYTES = 136;
 constexpr float M_UNIT = 0x1p-112f, V_UNIT = 0x1p-96f;       // 1.0 times these has the exponent fields 15 and 31: the largest codes
-constexpr unsigned M_TOP = 0x78, V_TOP = 0xF8;
 
-// The hash of a place and a step, its first line apart: four neighbouring places from a multiple of four on differ in it by their last two bits.
+// The hash of a place and a step, its first line apart: eight neighbouring places from a multiple of eight on differ in it by their last three bits.
 __device__ __forceinline__ unsigned random_seed(unsigned long long place, unsigned step) {
     return (unsigned)place ^ ((unsigned)(place >> 32) * 0x632BE5ABu) ^ (step * 0x9E3779B1u);
 }
@@ -117,109 +145,127 @@ __device__ __forceinline__ unsigned random32(unsigned x) {
     x = (x ^ (x >> 15)) * 0x6C8E9D73u;
     return x ^ (x >> 16);
 }
-__device__ __forceinline__ float decode_m(unsigned c, float largest) {
-    const float x = __fmul_rn(__fmul_rn(__uint_as_float((c & 127u) << 20), 1.f / M_UNIT), largest);
-    return c & 128u ? -x : x;
+// Two codes of m, from the places 2 k and 2 k + 1 of a word: with the exponent's bias of 7 that the conversion takes, 1.0 (the largest code there is) is
+// 256 of its units.
+__device__ __forceinline__ Two decode_m(unsigned word, int k, float top) {
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(word >> (16 * k))));
+    const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&h));
+    return mul2(mul2(Two{f.x, f.y}, both(0x1p-8f)), both(top));
 }
-__device__ __forceinline__ float decode_v(unsigned c, float largest) { return __fmul_rn(__fmul_rn(__uint_as_float(c << 20), 1.f / V_UNIT), largest); }
-__device__ __forceinline__ unsigned encode(float x, float inv, float unit, unsigned top, unsigned random16) {
-    return min((__float_as_uint(__fmul_rn(__fmul_rn(x, inv), unit)) + (random16 << 4)) >> 20, top);
+__device__ __forceinline__ Two decode_v(unsigned word, int k, float top) {
+    const unsigned a = k ? word << 4 : word << 20, b = k ? word >> 4 : word << 12;
+    return mul2(mul2(Two{__uint_as_float(a & 0x0ff00000u), __uint_as_float(b & 0x0ff00000u)}, both(1.f / V_UNIT)), both(top));
 }
-// A block whose largest entry is below the smallest normal float is held as zeros.
-__device__ __forceinline__ float largest_of(unsigned bits, float &inv) {
-    float x = __uint_as_float(bits);
+// An entry over the block's largest, in the units of the code, with the random bits added below the code's last place: the code is in the bits from 20
+// on (at most the largest code: 1.0 has zeros below).
+__device__ __forceinline__ Two scaled(Two x, float inv, float unit) { return mul2(mul2(x, both(inv)), both(unit)); }
+__device__ __forceinline__ unsigned rounded(float x, unsigned random16) { return __float_as_uint(x) + (random16 << 4); }
+// Byte 3 of each of four words
+__device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+// A block whose largest entry is below the smallest normal float is held as zeros.  (Infinity times the smallest number is infinity still, whose bits give
+// the largest code, and the finite entries beside it zeros.)
+__device__ __forceinline__ float held(float x, float &inv) {
     if (x < 1.17549435e-38f) x = 0.f;
-    inv = x > 0.f ? __frcp_rn(x) : 0.f;
+    inv = x > 0.f ? fmaxf(__frcp_rn(x), __uint_as_float(1u)) : 0.f;
     return x;
 }
 
+// A thread has EIGHT neighbouring entries, so eight threads share a block of 64.
+constexpr int EIGHT = 8;
+static_assert(CHUNK == EIGHT * THREADS, "one pass");
 __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__ AdamWTable tab, const __grid_constant__ AdamWArgs by_value) {
-    const AdamWTensor &t = tab.t[tensor_of(tab, blockIdx.x)];
+    const int number = tensor_of(tab, blockIdx.x);
+    const AdamWTensor &t = tab.t[number];
     const AdamWArgs a = adamw_args(tab, by_value, true);
-    const Update u = update_of(a, t.decay);
-    const unsigned step = (unsigned)a.step;
-    const long long at = (long long)(blockIdx.x - t.first) * CHUNK;
-    const int n = (int)min((long long)CHUNK, t.n - at);
-    float *w = t.w + at;
-    const float *g = t.g + at;
-    char *state = (char *)t.m + at / BLOCK_ENTRIES * BLOCK_BYTES;
-    const bool vec = !(((uintptr_t)w | (uintptr_t)g) & 15);
-    const int part = threadIdx.x & 15;                        // 16 threads a block of 64 entries
-    float ww[2][4], gg[2][4];
-    uint2 code[2];
-    float2 top[2];
+    const Update u = update_of(a, tab.decay[number]);
+    const long long at = (long long)(blockIdx.x - tab.first[number]) * CHUNK;
+    const int n = (int)min((long long)CHUNK, t.n - at), i = threadIdx.x * EIGHT;
+    float *w = t.w + at + i;
+    const float *g = t.g + at + i;
+    char *block = (char *)t.m + (at + i) / BLOCK_ENTRIES * BLOCK_BYTES;
+    uint2 *codes = (uint2 *)block + threadIdx.x % 8 * 2;
+    const bool there = i / BLOCK_ENTRIES * BLOCK_ENTRIES < n;             // the tensor's last block may be short, its codes are there for all 64
+    const bool whole = !(((uintptr_t)w | (uintptr_t)g) & 15) && i + EIGHT <= n;
+    Two ww[4] = {}, gg[4] = {}, m[4], v[4];
+    uint2 code[2] = {};
+    float2 top = make_float2(0.f, 0.f);
+    if (there) { code[0] = codes[0]; code[1] = codes[1]; top = *(const float2 *)(block + 128); }
+    if (whole) {
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int i = (threadIdx.x + k * THREADS) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; j++) ww[k][j] = gg[k][j] = 0.f;
-        code[k] = make_uint2(0, 0);
-        top[k] = make_float2(0.f, 0.f);
-        if (i / BLOCK_ENTRIES * BLOCK_ENTRIES < n) {          // the tensor's last block may be short, its codes are there for all 64
-            const char *blk = state + i / BLOCK_ENTRIES * BLOCK_BYTES;
-            code[k] = ((const uint2 *)blk)[part];
-            top[k] = *(const float2 *)(blk + 128);
+        for (int k = 0; k < 2; k++) {
+            const float4 x = ((const float4 *)w)[k], y = __ldcs((const float4 *)g + k);
+            ww[2 * k] = Two{x.x, x.y}; ww[2 * k + 1] = Two{x.z, x.w};
+            gg[2 * k] = Two{y.x, y.y}; gg[2 * k + 1] = Two{y.z, y.w};
         }
-        if (vec && i + 4 <= n) {
-            const float4 x = *(const float4 *)(w + i), y = __ldcs((const float4 *)(g + i));
-            ww[k][0] = x.x; ww[k][1] = x.y; ww[k][2] = x.z; ww[k][3] = x.w;
-            gg[k][0] = y.x; gg[k][1] = y.y; gg[k][2] = y.z; gg[k][3] = y.w;
-        } else {
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) if (i + j < n) { ww[k][j] = w[i + j]; gg[k][j] = g[i + j]; }
+        for (int j = 0; j < 4; j++) {
+            if (i + 2 * j < n) { ww[j].x = w[2 * j]; gg[j].x = g[2 * j]; }
+            if (i + 2 * j + 1 < n) { ww[j].y = w[2 * j + 1]; gg[j].y = g[2 * j + 1]; }
         }
     }
+    float am = 0.f, av = 0.f;                                 // a NaN is larger than all else, and its block shows it
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int i = (threadIdx.x + k * THREADS) * 4;
-        float m[4], v[4];
-        unsigned am = 0, av = 0;
+    for (int j = 0; j < 4; j++) {
+        m[j] = decode_m(code[j / 2].x, j % 2, top.x);
+        v[j] = decode_v(code[j / 2].y, j % 2, top.y);
+        adamw_two(ww[j], gg[j], m[j], v[j], a, u);
+        if (!whole) {                                         // places behind the tensor's end
+            if (i + 2 * j >= n) m[j].x = v[j].x = 0.f;
+            if (i + 2 * j + 1 >= n) m[j].y = v[j].y = 0.f;
+        }
+        am = largest(am, largest(fabsf(m[j].x), fabsf(m[j].y)));
+        av = largest(av, largest(v[j].x, v[j].y));
+    }
+#pragma unroll
+    for (int o = 4; o; o >>= 1) {
+        am = largest(am, __shfl_xor_sync(0xffffffffu, am, o));
+        av = largest(av, __shfl_xor_sync(0xffffffffu, av, o));
+    }
+    float im, iv;
+    const float lm = held(am, im), lv = held(av, iv);
+    const unsigned seed = random_seed((unsigned long long)(t.place + at + i), (unsigned)a.step);
+    unsigned qm[8], qv[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const unsigned r0 = random32(seed ^ (2 * j)), r1 = random32(seed ^ (2 * j + 1));
+        const Two sm = scaled(m[j], im, M_UNIT), sv = scaled(v[j], iv, V_UNIT);
+        qm[2 * j] = rounded(sm.x, r0 & 0xffffu); qm[2 * j + 1] = rounded(sm.y, r1 & 0xffffu);
+        qv[2 * j] = rounded(sv.x, r0 >> 16); qv[2 * j + 1] = rounded(sv.y, r1 >> 16);
+    }
+    if (there) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const unsigned *x = qm + 4 * k, *y = qv + 4 * k;
+            const unsigned size = top_bytes(x[0] << 4, x[1] << 4, x[2] << 4, x[3] << 4), sign = top_bytes(x[0], x[1], x[2], x[3]);
+            codes[k] = make_uint2((size & 0x7f7f7f7fu) | (sign & 0x80808080u), top_bytes(y[0] << 4, y[1] << 4, y[2] << 4, y[3] << 4));
+        }
+        if (threadIdx.x % 8 == 0) *(float2 *)(block + 128) = make_float2(lm, lv);
+    }
+    if (whole) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) ((float4 *)w)[k] = make_float4(ww[2 * k].x, ww[2 * k].y, ww[2 * k + 1].x, ww[2 * k + 1].y);
+    } else {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            m[j] = decode_m((code[k].x >> (8 * j)) & 255u, top[k].x);
-            v[j] = decode_v((code[k].y >> (8 * j)) & 255u, top[k].y);
-            adamw_one(ww[k][j], gg[k][j], m[j], v[j], a, u);
-            if (i + j >= n) m[j] = v[j] = 0.f;                // places behind the tensor's end
-            am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);      // as bits: a NaN is larger than all else, and its block shows it
-            av = max(av, __float_as_uint(v[j]) & 0x7fffffffu);
-        }
-#pragma unroll
-        for (int o = 8; o; o >>= 1) {
-            am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-            av = max(av, __shfl_xor_sync(0xffffffffu, av, o));
-        }
-        float im, iv;
-        const float lm = largest_of(am, im), lv = largest_of(av, iv);
-        uint2 c = make_uint2(0, 0);
-        const unsigned seed = random_seed((unsigned long long)(t.place + at + i), step);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const unsigned r = random32(seed ^ j);
-            c.x |= (encode(fabsf(m[j]), im, M_UNIT, M_TOP, r & 0xffffu) | (m[j] < 0.f ? 128u : 0u)) << (8 * j);
-            c.y |= encode(v[j], iv, V_UNIT, V_TOP, r >> 16) << (8 * j);
-        }
-        if (i / BLOCK_ENTRIES * BLOCK_ENTRIES < n) {
-            char *blk = state + i / BLOCK_ENTRIES * BLOCK_BYTES;
-            ((uint2 *)blk)[part] = c;
-            if (part == 0) *(float2 *)(blk + 128) = make_float2(lm, lv);
-        }
-        if (vec && i + 4 <= n) *(float4 *)(w + i) = make_float4(ww[k][0], ww[k][1], ww[k][2], ww[k][3]);
-        else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) if (i + j < n) w[i + j] = ww[k][j];
+            if (i + 2 * j < n) w[2 * j] = ww[j].x;
+            if (i + 2 * j + 1 < n) w[2 * j + 1] = ww[j].y;
         }
     }
 }
 
 __global__ void __launch_bounds__(256) adamw8_read_kernel(const char *__restrict__ state, float *__restrict__ m, float *__restrict__ v, long long n) {
     const bool vec = !(((uintptr_t)m | (uintptr_t)v) & 15);
-    for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p * 4 < n; p += (long long)gridDim.x * 256) {
+    const long long p = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (p * 4 < n) {
         const char *blk = state + p / 16 * BLOCK_BYTES;
         const uint2 c = ((const uint2 *)blk)[p & 15];
         const float2 top = *(const float2 *)(blk + 128);
-        float x[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) { x[j] = decode_m((c.x >> (8 * j)) & 255u, top.x); y[j] = decode_v((c.y >> (8 * j)) & 255u, top.y); }
+        const Two x0 = decode_m(c.x, 0, top.x), x1 = decode_m(c.x, 1, top.x), y0 = decode_v(c.y, 0, top.y), y1 = decode_v(c.y, 1, top.y);
+        const float x[4] = {x0.x, x0.y, x1.x, x1.y}, y[4] = {y0.x, y0.y, y1.x, y1.y};
         const long long i = p * 4;
         if (vec && i + 4 <= n) {
             *(float4 *)(m + i) = make_float4(x[0], x[1], x[2], x[3]);
@@ -255,8 +301,10 @@ int adamw(bool eight, int count, float *const *w, const float *const *g, void *c
             if (n[i] == 0) continue;
             const long long need = (n[i] + CHUNK - 1) / CHUNK;
             if (blocks + need > 0x7fffffffLL) break;
+            table->first[table->count] = (unsigned)blocks;
+            table->decay[table->count] = decay[i];
             AdamWTensor &t = table->t[table->count++];
-            t.w = w[i]; t.g = g[i]; t.m = m[i]; t.n = n[i]; t.decay = decay[i]; t.first = (unsigned)blocks;
+            t.w = w[i]; t.g = g[i]; t.m = m[i]; t.n = n[i];
             if (eight) t.place = first;
             else t.v = v[i];
             blocks += need;
@@ -306,8 +354,9 @@ int seera_adamw8_step(int count, float *const *w, const float *const *g, void *c
 int seera_adamw8_read(const void *state, float *m, float *v, long long n) {
     SEERA_ENSURE();
     if (n < 0 || (n > 0 && (!state || !m || !v)) || ((uintptr_t)state & 7)) return fail(SEERA_E_ARG, "adamw8_read: bad argument");
+    if (n > (1LL << 40)) return fail(SEERA_E_LIMIT, "adamw8_read: %lld entries", n);
     if (n == 0) return SEERA_OK;
-    adamw8_read_kernel<<<stride_grid((n + 3) / 4), 256, 0, rt().stream>>>((const char *)state, m, v, n);
+    adamw8_read_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, rt().stream>>>((const char *)state, m, v, n);
     SEERA_LAUNCH_CHECK("adamw8_read");
     return SEERA_OK;
 }

@@ -9,6 +9,7 @@
 //
 // Steps at and behind a sequence's length hold the state, write zeros and are not read.
 #include "common.cuh"
+#include "pairs.cuh"
 #include "sigmoid.cuh"
 #include "tc_ptx.cuh"
 #include <initializer_list>
@@ -43,8 +44,6 @@ constexpr float HOLD = 0.f;                               // the gate of a step 
 __device__ __forceinline__ bool keeps(float s) { return __float_as_int(s) >= 0; }       // (the sign of a zero counts)
 // a h + (1 - a) v = h + s (v - h) or v - s (v - h)
 __device__ __forceinline__ float step_of(float s, float h, float v) { return fmaf(s, v - h, keeps(s) ? h : v); }
-// a x = x - s x or s x
-__device__ __forceinline__ float decay(float s, float x) { return fmaf(-s, x, keeps(s) ? x : 0.f); }
 // a x and (1 - a) x
 __device__ __forceinline__ void part(float s, float x, float &a_x, float &na_x) {
     const float y = fabsf(s) * x, z = x - y;
@@ -114,26 +113,6 @@ __global__ void __launch_bounds__(128) scan_bwd_serial_kernel(const __grid_const
 // 2048 x 2048 148 us (5.4 TB/s).  A lane with one channel and 16 steps took 80, 137 and 148 us, and a tile of 64 channels 102, 220 and 162.
 constexpr int MAX_RANKS = 16, STAGES = 3, TILE = 32, WARPS = 8, FWD_STEPS = 8, BWD_STEPS = 4;
 
-struct __align__(8) Two { float x, y; };                  // a lane's two channels
-__device__ __forceinline__ unsigned long long bits(Two a) { return *reinterpret_cast<unsigned long long *>(&a); }
-__device__ __forceinline__ Two two(unsigned long long b) { return *reinterpret_cast<Two *>(&b); }
-__device__ __forceinline__ Two both(float x) { return Two{x, x}; }
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-    return two(d);
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-    return two(d);
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-    unsigned long long d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-    return two(d);
-}
-__device__ __forceinline__ Two less2(Two a, Two b) { return fma2(b, both(-1.f), a); }       // a - b
 __device__ __forceinline__ Two pick(bool kx, bool ky, Two a, Two b) { return Two{kx ? a.x : b.x, ky ? a.y : b.y}; }
 // sigmoid_less of two, bit for bit
 __device__ __forceinline__ Two sigmoid_less2(Two f) {
