@@ -134,7 +134,7 @@ __device__ __forceinline__ Run no_steps() { return Run{both(1.f), both(0.f)}; }
 __device__ __forceinline__ Two after(const Run &r, Two x) { return fma2(r.a, x, r.b); }
 __device__ __forceinline__ Run then(const Run &first, const Run &second) { return Run{mul2(first.a, second.a), after(second, first.b)}; }
 template <int W> struct Joined {
-    Run warps[2][W][16], ranks[2][MAX_RANKS][16];
+    Run warps[3][W][16], ranks[2][MAX_RANKS][16];
     Two carry[2][16];
     unsigned long long bar[2];
 };
@@ -178,7 +178,7 @@ template <int W, int L> struct Place {
     int warp, lane, half, col, rank, ranks, n, c0, c, len, piece, first;
     bool on, on2;                                          // whether the lane's channels are there
     Waits waits;
-    Two carry;                                             // several blocks: the state at the start of the piece (one block has it in shared memory)
+    Two carry;                                             // several blocks: the state at the start of the piece, in the warp that takes it in
     template <class P> __device__ __forceinline__ Place(const P &p, Joined<W> &sm_) : sm(sm_) {
         warp = threadIdx.x >> 5; lane = threadIdx.x & 31; half = lane >> 4; col = lane & 15; ranks = p.ranks; rank = blockIdx.x % ranks;
         const unsigned tiles = (p.C + TILE - 1) / TILE, tile = blockIdx.x / ranks;
@@ -208,50 +208,53 @@ template <int W, int L> struct Place {
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    // What the thread's steps of piece k do to a state (`run`) is given out.  Afterwards `run` is what the warp's other half does in front of it.
+    // What the thread's steps of piece k do to a state (`run`): its warp's goes to shared memory, and `run` is then what the warp's other half does in
+    // front of it.  A barrier of the block follows, then pass_on.
     __device__ __forceinline__ void give(int k, Run &run) {
-        const int buf = k & 1;
         Run other;
         other.a = two(__shfl_xor_sync(0xffffffffu, bits(run.a), 16));
         other.b = two(__shfl_xor_sync(0xffffffffu, bits(run.b), 16));
-        if (!half) sm.warps[buf][warp][col] = then(run, other);
+        if (!half) sm.warps[k % 3][warp][col] = then(run, other);
         run = half ? other : no_steps();
-        __syncthreads();
-        if (ranks > 1) {
-            Run all = sm.warps[buf][0][col];
+    }
+    // The block's steps of piece k, sent to every block of the cluster by one warp.
+    __device__ __forceinline__ void pass_on(int k) {
+        if (ranks == 1 || warp != 0) return;
+        const int buf = k & 1;
+        const Run *runs = &sm.warps[k % 3][0][col];
+        Run all = runs[0];
 #pragma unroll
-            for (int i = 1; i < W; i++) all = then(all, sm.warps[buf][i][col]);
-            if (threadIdx.x == 0)
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&sm.bar[buf])), "r"(ranks * 16 * (int)sizeof(Run)) : "memory");
-            for (int r = 2 * warp + half; r < ranks; r += 2 * W) send(&sm.ranks[buf][rank][col], &sm.bar[buf], r, all);
-        }
+        for (int i = 1; i < W; i++) all = then(all, runs[16 * i]);
+        if (threadIdx.x == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&sm.bar[buf])), "r"(ranks * 16 * (int)sizeof(Run)) : "memory");
+        for (int r = half; r < ranks; r += 2) send(&sm.ranks[buf][rank][col], &sm.bar[buf], r, all);
+    }
+    // The state at the start of the block's steps of piece k, put into shared memory by another warp.  A barrier of the block follows, then start.
+    __device__ __forceinline__ void take_in(int k) {
+        if (ranks == 1 || warp != 1) return;
+        const int buf = k & 1;
+        await(smem_u32(&sm.bar[buf]), (k >> 1) & 1, waits);
+#pragma unroll 4
+        for (int r = 0; r < rank; r++) carry = after(sm.ranks[buf][r][col], carry);
+        if (!half) sm.carry[buf][col] = carry;
+#pragma unroll 4
+        for (int r = rank; r < ranks; r++) carry = after(sm.ranks[buf][r][col], carry);
     }
     // The state at the start of the thread's steps of piece k.
-    __device__ __forceinline__ Two receive(int k, const Run &before) {
-        const int buf = k & 1;
-        Two x;
-        if (ranks > 1) {
-            await(smem_u32(&sm.bar[buf]), (k >> 1) & 1, waits);
-            x = carry;
-#pragma unroll 4
-            for (int r = 0; r < rank; r++) x = after(sm.ranks[buf][r][col], x);
-            carry = x;
-#pragma unroll 4
-            for (int r = rank; r < ranks; r++) carry = after(sm.ranks[buf][r][col], carry);
-        } else {
-            x = sm.carry[buf][col];
-        }
+    __device__ __forceinline__ Two start(int k, const Run &before) {
+        Two x = sm.carry[k & 1][col];
+        const Run *runs = &sm.warps[k % 3][0][col];
 #pragma unroll
         for (int i = 0; i < W - 1; i++)
-            if (i < warp) x = after(sm.warps[buf][i][col], x);
-        if (ranks == 1 && warp == W - 1 && !half) sm.carry[buf ^ 1][col] = after(sm.warps[buf][W - 1][col], x);
+            if (i < warp) x = after(runs[16 * i], x);
+        if (ranks == 1 && warp == W - 1 && !half) sm.carry[(k + 1) & 1][col] = after(runs[16 * (W - 1)], x);
         return after(before, x);
     }
     // The state behind the last of k pieces goes to `last`.  No block leaves while another may still send to it: every block has waited for all
     // that is sent to it, which the cluster's barrier makes sure of where a wait has run out.
     __device__ __forceinline__ void end(int k, float *last, int C) {
         if (ranks == 1) __syncthreads();
-        if (last && rank == 0 && threadIdx.x < 16) {
+        if (last && rank == 0 && warp == (ranks > 1) && !half) {
             if (ranks == 1) carry = sm.carry[k & 1][col];
             const long long i = (long long)n * C + c;
             if (on) last[i] = carry.x;
@@ -346,20 +349,33 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
         }
     };
     int k = 0;
-    auto go = [&](const Run (&now)[L], Run (&next)[L]) {    // `now` has been worked on
-        Run before = now[L - 1];
-        me.give(k, before);
-        work(next, t0 + me.piece);                          // (while the others' runs are on their way)
-        write(now, me.receive(k, before), t0);
+    Run before;
+    auto go = [&](const Run (&now)[L], Run (&next)[L], bool more) {       // `now` has been worked on and its runs are passed on
+        Run then_before;
+        if (more) {
+            work(next, t0 + me.piece);                      // (while the others' runs are on their way)
+            then_before = next[L - 1];
+            me.give(k + 1, then_before);
+        }
+        me.take_in(k);
+        __syncthreads();
+        if (more) me.pass_on(k + 1);
+        write(now, me.start(k, before), t0);
+        before = then_before;
         t0 += me.piece;
         k++;
     };
     Run one[L], two[L];
     work(one, t0);
+    before = one[L - 1];
+    me.give(0, before);
+    __syncthreads();
+    me.pass_on(0);
     for (long long start = 0; start < p.T; start += 2 * me.piece) {
-        go(one, two);
-        if (start + me.piece >= p.T) break;
-        go(two, one);
+        const bool more = start + me.piece < p.T;
+        go(one, two, more);
+        if (!more) break;
+        go(two, one, start + 2 * me.piece < p.T);
     }
     me.end(k, p.last, p.C);
 }
@@ -419,7 +435,11 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
         if (t0 > 0 && t0 + Me::STEPS <= me.len) work(true);
         else work(false);
         me.give(k, run);
-        Two x = me.receive(k, run);
+        __syncthreads();
+        me.pass_on(k);
+        me.take_in(k);
+        if (me.ranks > 1) __syncthreads();
+        Two x = me.start(k, run);
         const int t1 = t0 + own;
         if (me.on && t1 + L > 0) {
             float *pf = p.df + (at + t1 + L - 1) * p.ldg + me.c, *pv = p.dv + (at + t1 + L - 1) * p.ldg + me.c;
