@@ -235,6 +235,8 @@ class _NormGrad:
         self.dy, self.norm, self.plain = dy, norm, None
 
     def add(self, g):
+        if isinstance(g, _PooledGrad):
+            g = g.materialize()
         if self.plain is not None:
             out = _new(g.shape)
             sc.cuda_elemadd(self.plain.main_ptr, g.main_ptr, out.main_ptr, g.size)

@@ -223,3 +223,75 @@ def test_offsets_past_32_bits(D):
         capi.check(d.L.seera_gated_scan_fwd(big, big + 64, ld, d.up(h0), None, h, None, N, T, C))
         assert (np.abs(d.down(h, (N, T, C)) - want) <= eh).all()
     capi.check(capi.load().seera_pool_trim())
+
+
+# Channels and rows of whole vectors, which are copied 16 bytes at a time: one block a tile, clusters of a few blocks and of as many as there are
+WIDE = [(3, 17, 64), (1, 129, 4), (5, 64, 32), (2, 300, 100), (7, 255, 68), (300, 40, 36), (40, 300, 128), (3, 2049, 40), (1, 5000, 256), (1, 12000, 64), (2, 3001, 512)]
+
+
+@pytest.mark.parametrize("N,T,C", WIDE)
+@pytest.mark.parametrize("state,ragged,given", [(False, False, "dh"), (True, True, "both"), (True, False, "dlast")])
+def test_whole_vectors(D, N, T, C, state, ragged, given):
+    Dev, capi = D
+    f, v, h0, dh, dlast, lengths = inputs(N, T, C, N + 3 * T + C, ragged)
+    want, last, eh, elast = ref.scan_fwd(f, v, h0 if state else None, lengths)
+    h32 = want.astype(np.float32)
+    use_dh, use_last = given != "dlast", given != "dh"
+    df, dv, dh0, edf, edv, edh0 = ref.scan_bwd(f, v, h32, dh if use_dh else None, dlast if use_last else None, h0 if state else None, lengths)
+    with Dev() as d:
+        ld, ldg = 2 * C + 4, 2 * C + 2
+        z = d.up(poison(joined(f, v, 4), lengths))
+        h, hl = Guarded(d, N * T * C), Guarded(d, N * C)
+        args = (z, z + 4 * C, ld, d.up(h0) if state else None, d.up(lengths, np.int32) if ragged else None)
+        capi.check(d.L.seera_gated_scan_fwd(*args, h.at, hl.at, N, T, C))
+        got, gl = h.get((N, T, C)), hl.get((N, C))
+        assert (np.abs(got - want) <= eh).all() and (np.abs(gl - last) <= elast).all()
+        if ragged:
+            assert all((got[n, k:] == 0).all() for n, k in enumerate(lengths))
+        out, o0 = Guarded(d, N * T * ldg), Guarded(d, N * C)
+        args += (d.up(poison(h32.copy(), lengths)), d.up(poison(dh.copy(), lengths)) if use_dh else None, d.up(dlast) if use_last else None)
+        capi.check(d.L.seera_gated_scan_bwd(*args, out.at, out.at + 4 * C, ldg, o0.at, N, T, C))
+        got, g0 = out.get((N, T, ldg)), o0.get((N, C))
+        assert (got[..., 2 * C:] == 7.5).all()                                          # between the rows of the gradient
+        assert (np.abs(got[..., :C] - df) <= edf).all() and (np.abs(got[..., C:2 * C] - dv) <= edv).all() and (np.abs(g0 - dh0) <= edh0).all()
+        if ragged:
+            assert all((got[n, k:, :2 * C] == 0).all() for n, k in enumerate(lengths))
+        capi.check(d.L.seera_gated_scan_bwd(*args, out.at, out.at + 4 * C, ldg, None, N, T, C))
+        assert np.array_equal(out.get((N, T, ldg)), got)
+        assert d.L.seera_tc_device_status() == 0
+
+
+@pytest.mark.parametrize("N,T,C", [(1, 4000, 64), (2, 777, 33)])
+def test_two_recordings_share_nothing(D, N, T, C):
+    """Two recordings of forward and backward calls of clusters, replayed in turn with other inputs in place of their own."""
+    Dev, capi = D
+    with Dev() as d:
+        runs = []
+        for seed in (1, 2):
+            f, v, h0, dh, dlast, lengths = inputs(N, T, C, seed, True)
+            a = {"f": d.up(f), "v": d.up(v), "h0": d.up(h0), "dh": d.up(dh), "len": d.up(lengths, np.int32)}
+            a.update(h=d.new(N * T * C), last=d.new(N * C), df=d.new(N * T * C), dv=d.new(N * T * C), dh0=d.new(N * C))
+            capi.check(d.L.seera_graph_begin())
+            capi.check(d.L.seera_gated_scan_fwd(a["f"], a["v"], C, a["h0"], a["len"], a["h"], a["last"], N, T, C))
+            capi.check(d.L.seera_gated_scan_bwd(a["f"], a["v"], C, a["h0"], a["len"], a["h"], a["dh"], a["last"], a["df"], a["dv"], C, a["dh0"], N, T, C))
+            g = d.L.seera_graph_end()
+            assert g
+            runs.append((a, g))
+        for seed in (3, 4, 5):
+            data = [inputs(N, T, C, 10 * seed + i, True) for i in range(2)]
+            for (a, g), (f, v, h0, dh, _, lengths) in zip(runs, data):
+                for k, x in (("f", f), ("v", v), ("h0", h0), ("dh", dh)):
+                    capi.check(d.L.seera_cuda_memcopy_devicetodevice(a[k], d.up(x), x.size))
+                capi.check(d.L.seera_cuda_memcopy_devicetodevice(a["len"], d.up(lengths, np.int32), N))
+            for _, g in runs:
+                capi.check(d.L.seera_graph_launch(g))
+            for (a, g), (f, v, h0, dh, _, lengths) in zip(runs, data):
+                want, last, eh, elast = ref.scan_fwd(f, v, h0, lengths)
+                got, gl = d.down(a["h"], (N, T, C)), d.down(a["last"], (N, C))
+                assert (np.abs(got - want) <= eh).all() and (np.abs(gl - last) <= elast).all()
+                df, dv, dh0, edf, edv, edh0 = ref.scan_bwd(f, v, got, dh, gl, h0, lengths)
+                for k, w, e in (("df", df, edf), ("dv", dv, edv), ("dh0", dh0, edh0)):
+                    assert (np.abs(d.down(a[k], w.shape) - w) <= e).all()
+        for _, g in runs:
+            capi.check(d.L.seera_graph_destroy(g))
+        assert d.L.seera_tc_device_status() == 0

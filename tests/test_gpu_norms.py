@@ -200,3 +200,36 @@ def test_gates_far_out(D, act):
     for k in ("du", "dres", "dgate", "dgamma"):
         assert np.isfinite(bwd[k]).all()
     close(bwd["dres"], wb["dres"], "dres")
+
+
+def test_norms_in_two_recordings(D):
+    """Forward and backward recorded twice, replayed in turn with other rows: each recording's sums over the blocks are its own."""
+    Dev, capi = D
+    rows, C = 700, 516
+    with Dev() as d:
+        runs = []
+        for _ in range(2):
+            a = {k: d.new(rows * C) for k in ("u", "g", "res", "dout", "dy", "out", "y", "du", "dgate", "dres")}
+            a.update({k: d.new(C) for k in ("gamma", "scale", "gamma2", "beta2", "dgamma", "dscale", "dgamma2", "dbeta2")}, st=d.new(4 * rows))
+            capi.check(d.L.seera_graph_begin())
+            capi.check(d.L.seera_gated_residual_fwd(a["u"], a["g"], C, a["res"], a["gamma"], a["scale"], a["out"], a["gamma2"], a["beta2"], a["y"], a["st"],
+                                                    rows, C, ref.LAYER, ref.SILU, ref.RMS, EPS, EPS))
+            capi.check(d.L.seera_gated_residual_bwd(a["dout"], a["dy"], a["u"], a["g"], C, a["res"], a["gamma"], a["scale"], a["gamma2"], a["st"], a["du"],
+                                                    a["dgate"], C, a["dres"], a["dgamma"], a["dscale"], a["dgamma2"], a["dbeta2"], rows, C, ref.LAYER, ref.SILU,
+                                                    ref.RMS))
+            g = d.L.seera_graph_end()
+            assert g
+            runs.append((a, g))
+        for seed in (1, 2):
+            data = [residual_inputs(rows, C, 10 * seed + i) for i in range(2)]
+            for (a, _), x in zip(runs, data):
+                for k, host in x.items():
+                    capi.check(d.L.seera_cuda_memcopy_devicetodevice(a[k], d.up(host), host.size))
+            for _, g in runs:
+                capi.check(d.L.seera_graph_launch(g))
+            for (a, _), x in zip(runs, data):
+                fwd, bwd = run_residual(D, rows, C, x, ref.LAYER, ref.SILU, ref.RMS)            # the same calls one by one
+                for k, want in [("out", fwd[0]), ("y", fwd[1])] + list(bwd.items()):
+                    assert np.array_equal(d.down(a[k], want.shape), want), k
+        for _, g in runs:
+            capi.check(d.L.seera_graph_destroy(g))
