@@ -104,14 +104,16 @@ __global__ void __launch_bounds__(128) scan_bwd_serial_kernel(const __grid_const
 // time.  What a run of steps does to a state is one multiply-add, x -> A x + B.  A thread forms it for each of its steps from its first one on; warps put
 // theirs into shared memory, blocks send theirs to the others of the cluster; with the state at its start every step is one multiply-add more.
 // A warp copies its own steps into its own part of shared memory, STAGES - 1 pieces ahead: nothing waits for another warp's data, and the loads
-// cost neither registers nor, with 16 bytes a copy, more than a quarter of an instruction an element.  One barrier of the block a piece.
+// cost neither registers nor, with 16 bytes a copy, more than a quarter of an instruction an element.  (A third stage gained nothing.)
 // Between blocks the runs travel by stores that count their bytes on a barrier in the receiver's shared memory (a barrier of the cluster would wait for
-// every result written before it).  Two places are used in turn: who writes one for the second next piece has received everybody's run of the next
-// one, which each sends after all of its warps have read the place.
-// Measured (fp32, inputs beyond L2): forward of 8 x 2048 x 2048 76 us (5.3 TB/s, bytes bound it), of one sequence of 65536 x 512 108 us (3.7 TB/s;
-// with 13 blocks of 256 threads a tile the SMs wait for one another's runs and on shared memory, 36 % of the issue slots are used); backward of 8 x
-// 2048 x 2048 148 us (5.4 TB/s).  A lane with one channel and 16 steps took 80, 137 and 148 us, and a tile of 64 channels 102, 220 and 162.
-constexpr int MAX_RANKS = 16, STAGES = 3, TILE = 32, WARPS = 8, FWD_STEPS = 8, BWD_STEPS = 4;
+// every result written before it); one warp sends and another takes in, since each warp that went through the other blocks' runs itself would read more
+// of them from shared memory than data.  Two places are used in turn: who writes one for the second next piece has received everybody's run of the
+// next one, which each sends after it has read the place.
+// Measured (fp32, inputs beyond L2): forward of 8 x 2048 x 2048 78 us (5.2 TB/s, the bytes), of one sequence of 65536 x 512 93 us (4.3 TB/s; 13 blocks
+// a tile, two an SM, leave a quarter of the SMs idle, and the others wait for one another's runs); backward of 8 x 2048 x 2048 148 us (5.4 TB/s).  With all
+// warps sending and taking in the second took 108 us; a lane with one channel and 16 steps took 80, 137 and 148 us, a tile of 64 channels 102, 220 and 162.
+// Rows that start anywhere, 7 x 1023 x 645 backward: 28 us, 39 with copies of single words, 76 with loads into registers.
+constexpr int MAX_RANKS = 16, STAGES = 2, TILE = 32, WARPS = 8, FWD_STEPS = 8, BWD_STEPS = 4;
 
 __device__ __forceinline__ Two pick(bool kx, bool ky, Two a, Two b) { return Two{kx ? a.x : b.x, ky ? a.y : b.y}; }
 // sigmoid_less of two, bit for bit
@@ -163,19 +165,24 @@ __device__ __forceinline__ void await(uint32_t bar, uint32_t parity, Waits &w) {
             return;
         }
 }
-// Copies of BYTES bytes from global into shared memory that the thread does not wait for.
-template <int BYTES> __device__ __forceinline__ void copy_async(float *to, const float *from) {
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+// A copy of 16 bytes from global into shared memory that the thread does not wait for.
+__device__ __forceinline__ void copy_async(float *to, const float *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
 
 // Which channels, steps and sequence a thread has, and how its runs and those of others are joined.
-template <int W, int L> struct Place {
-    static constexpr int STEPS = 2 * L, ROWS = STEPS * TILE;        // of a warp, and the floats of a tensor that it copies of a piece
+// VEC: whether rows start on 16 bytes and hold whole ones.  Where they do not, the whole 16 bytes that hold a row's part of the tile are copied, up to three
+// floats of what lies beside it with it (16 bytes that hold a float of a tensor belong to its allocation).
+template <int W, int L, bool VEC> struct Place {
+    static constexpr int STEPS = 2 * L;                    // of a warp
+    // Floats from row to row in shared memory, those that keep the half-warps' rows on different banks, and those of a tensor that a warp copies of a piece
+    static constexpr int WIDTH = VEC ? TILE : TILE + 4, GAP = VEC || L * WIDTH % 32 ? 0 : 16, ROWS = STEPS * WIDTH + GAP;
+    // One lane has two neighbouring channels, or two that are 16 apart, which single words are read and written side by side with.
+    static constexpr int APART = VEC ? 1 : 16;
     Joined<W> &sm;
-    int warp, lane, half, col, rank, ranks, n, c0, c, len, piece, first;
+    int warp, lane, half, col, in, rank, ranks, n, c0, c, len, piece, first;       // in: the place of the lane's first channel in its tile
     bool on, on2;                                          // whether the lane's channels are there
     Waits waits;
     Two carry;                                             // several blocks: the state at the start of the piece, in the warp that takes it in
@@ -184,8 +191,9 @@ template <int W, int L> struct Place {
         const unsigned tiles = (p.C + TILE - 1) / TILE, tile = blockIdx.x / ranks;
         n = tile / tiles;
         c0 = (tile - n * tiles) * TILE;
-        c = c0 + 2 * col;
-        on = c < p.C; on2 = c + 1 < p.C;
+        in = VEC ? 2 * col : col;
+        c = c0 + in;
+        on = c < p.C; on2 = c + APART < p.C;
         len = length_of(p.lengths, n, p.T);
         piece = ranks * W * STEPS;
         first = (rank * W + warp) * STEPS;
@@ -193,7 +201,7 @@ template <int W, int L> struct Place {
     }
     __device__ __forceinline__ Two state(const float *p, int C) const {
         const long long i = (long long)n * C + c;
-        return Two{on && p ? p[i] : 0.f, on2 && p ? p[i + 1] : 0.f};
+        return Two{on && p ? p[i] : 0.f, on2 && p ? p[i + APART] : 0.f};
     }
     __device__ __forceinline__ void begin(Two x) {
         carry = x;
@@ -258,42 +266,61 @@ template <int W, int L> struct Place {
             if (ranks == 1) carry = sm.carry[k & 1][col];
             const long long i = (long long)n * C + c;
             if (on) last[i] = carry.x;
-            if (on2) last[i + 1] = carry.y;
+            if (on2) last[i + APART] = carry.y;
         }
         if (ranks == 1) return;
         __syncwarp();
         asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     }
-    // Steps t0 .. t0 + STEPS - 1 of a tensor whose rows are `ld` floats apart into to[STEPS][TILE], those of them in [lo, len); `from`: where row t0 of
-    // this sequence and channel 0 are.
-    template <int BYTES> __device__ __forceinline__ void copy(float *to, const float *from, int t0, long long ld, int lo, int C) const {
-        constexpr int PER = BYTES / 4, ACROSS = TILE / PER, DOWN = 32 / ACROSS;
-        const int x = lane % ACROSS * PER, y = lane / ACROSS;
-        if (c0 + x >= C) return;
-        const float *p = from + y * ld + c0 + x;
-        float *t = to + y * TILE + x;
-        if (t0 >= lo && t0 + STEPS <= len) {
+    // Steps t0 .. t0 + STEPS - 1 of a tensor whose rows are `ld` floats apart into shared memory, those of them in [lo, len); `from`: where row t0 of
+    // this sequence and the tile's first channel are.
+    __device__ __forceinline__ void copy(float *to, const float *from, int t0, long long ld, int lo, int C) const {
+        if constexpr (VEC) {
+            constexpr int ACROSS = TILE / 4, DOWN = 32 / ACROSS;
+            const int x = lane % ACROSS * 4, y = lane / ACROSS;
+            if (c0 + x >= C) return;
+            const float *p = from + y * ld + x;
+            float *t = to + y * TILE + x;
+            if (t0 >= lo && t0 + STEPS <= len) {
 #pragma unroll
-            for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld) copy_async<BYTES>(t + i * TILE, p);
+                for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld) copy_async(t + i * TILE, p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld)
+                    if (t0 + i + y >= lo && t0 + i + y < len) copy_async(t + i * TILE, p);
+            }
         } else {
+            constexpr int ACROSS = WIDTH / 4;
+            const int width = min(TILE, C - c0);
 #pragma unroll
-            for (int i = 0; i < STEPS; i += DOWN, p += DOWN * ld)
-                if (t0 + i + y >= lo && t0 + i + y < len) copy_async<BYTES>(t + i * TILE, p);
+            for (int i = 0; i < STEPS * ACROSS; i += 32) {
+                const int y = (i + lane) / ACROSS, x = (i + lane) % ACROSS * 4;
+                const float *p = from + y * ld;
+                const int before = shift(p);
+                if (y < STEPS && t0 + y >= lo && t0 + y < len && x < before + width) copy_async(row(to, y) + x, p - before + x);
+            }
         }
     }
-    // The lane's channels to row `p` points to; pairs where PAIRS says that they lie on 8 bytes.
-    template <bool PAIRS> __device__ __forceinline__ void put(float *p, Two v) const {
-        if (PAIRS) {
+    __device__ __forceinline__ static int shift(const float *p) { return VEC ? 0 : (int)((uintptr_t)p >> 2 & 3); }
+    __device__ __forceinline__ static float *row(float *rows, int y) { return rows + y * WIDTH + (y >= L ? GAP : 0); }
+    // The lane's channels of the i-th of its half's L steps, where `shift` of that row is `before` (from: the half's first row), and to a row in global memory.
+    __device__ __forceinline__ Two get(const float *from, int i, int before) const {
+        const float *p = from + i * WIDTH + before + in;
+        if (VEC) return *reinterpret_cast<const Two *>(p);
+        return Two{p[0], p[APART]};
+    }
+    __device__ __forceinline__ void put(float *p, Two v) const {
+        if (VEC) {
             __stcs(reinterpret_cast<float2 *>(p), make_float2(v.x, v.y));
         } else {
             __stcs(p, v.x);
-            if (on2) __stcs(p + 1, v.y);
+            if (on2) __stcs(p + APART, v.y);
         }
     }
 };
 
-template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 / W) scan_fwd_kernel(const __grid_constant__ ScanFwd p) {
-    typedef Place<W, L> Me;
+template <int W, int L, bool VEC> __global__ void __launch_bounds__(W * 32, 16 / W) scan_fwd_kernel(const __grid_constant__ ScanFwd p) {
+    typedef Place<W, L, VEC> Me;
     constexpr int ROWS = Me::ROWS;
     __shared__ Joined<W> sm;
     extern __shared__ __align__(16) float stages[];         // [STAGES][W][f, v][2 L][TILE]
@@ -303,8 +330,8 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
     auto request = [&](int t0, int stage) {
         float *to = mine + stage * W * 2 * ROWS;
         if (t0 < me.len) {
-            me.template copy<BYTES>(to, p.f + (at + t0) * p.ld, t0, p.ld, 0, p.C);
-            me.template copy<BYTES>(to + ROWS, p.v + (at + t0) * p.ld, t0, p.ld, 0, p.C);
+            me.copy(to, p.f + (at + t0) * p.ld + me.c0, t0, p.ld, 0, p.C);
+            me.copy(to + ROWS, p.v + (at + t0) * p.ld + me.c0, t0, p.ld, 0, p.C);
         }
         copies_commit();
     };
@@ -317,14 +344,15 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
         copies_wait();
         __syncwarp();                                       // the piece is there for every lane, and the stage before it is read
         request(t0 + (STAGES - 1) * me.piece, stage == 0 ? STAGES - 1 : stage - 1);
-        const float *from = mine + stage * W * 2 * ROWS + own * TILE + 2 * me.col;
+        const float *from = Me::row(mine + stage * W * 2 * ROWS, own);
+        const float *pf = p.f + (at + t0 + own) * p.ld + me.c0, *pv = p.v + (at + t0 + own) * p.ld + me.c0;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         auto steps = [&](bool all) {
             Run run = no_steps();
 #pragma unroll
             for (int i = 0; i < L; i++) {
                 if (all || t0 + own + i < me.len) {
-                    const Two f = *reinterpret_cast<const Two *>(from + i * TILE), v = *reinterpret_cast<const Two *>(from + ROWS + i * TILE), s = sigmoid_less2(f);
+                    const Two f = me.get(from, i, Me::shift(pf + i * p.ld)), v = me.get(from + ROWS, i, Me::shift(pv + i * p.ld)), s = sigmoid_less2(f);
                     const bool kx = keeps(s.x), ky = keeps(s.y);
                     run.b = fma2(s, less2(v, run.b), pick(kx, ky, run.b, v));
                     run.a = fma2(Two{-s.x, -s.y}, run.a, pick(kx, ky, run.a, both(0.f)));
@@ -341,11 +369,11 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
         float *h = p.h + (at + t0) * p.C + me.c;
         if (t0 + L <= me.len) {
 #pragma unroll
-            for (int i = 0; i < L; i++, h += p.C) me.template put<BYTES == 16>(h, after(m[i], x));
+            for (int i = 0; i < L; i++, h += p.C) me.put(h, after(m[i], x));
         } else {
 #pragma unroll
             for (int i = 0; i < L; i++, h += p.C)
-                if (t0 + i < p.T) me.template put<BYTES == 16>(h, t0 + i < me.len ? after(m[i], x) : both(0.f));
+                if (t0 + i < p.T) me.put(h, t0 + i < me.len ? after(m[i], x) : both(0.f));
         }
     };
     int k = 0;
@@ -381,8 +409,8 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
 }
 
 // Backward: the same with time running from the end, where c -> a (dh + c) is what a step does.
-template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 / W) scan_bwd_kernel(const __grid_constant__ ScanBwd p) {
-    typedef Place<W, L> Me;
+template <int W, int L, bool VEC> __global__ void __launch_bounds__(W * 32, 16 / W) scan_bwd_kernel(const __grid_constant__ ScanBwd p) {
+    typedef Place<W, L, VEC> Me;
     constexpr int ROWS = Me::ROWS;
     __shared__ Joined<W> sm;
     extern __shared__ __align__(16) float stages[];         // [STAGES][W][f, v, dh, h of the step before][2 L][TILE]
@@ -392,10 +420,10 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
     auto request = [&](int t0, int stage) {                 // steps t0 .. t0 + 2 L - 1, of which some may lie before the first
         float *to = mine + stage * W * 4 * ROWS;
         if (t0 + Me::STEPS > 0 && t0 < me.len) {
-            me.template copy<BYTES>(to, p.f + (at + t0) * p.ld, t0, p.ld, 0, p.C);
-            me.template copy<BYTES>(to + ROWS, p.v + (at + t0) * p.ld, t0, p.ld, 0, p.C);
-            if (p.dh) me.template copy<BYTES>(to + 2 * ROWS, p.dh + (at + t0) * p.C, t0, p.C, 0, p.C);
-            me.template copy<BYTES>(to + 3 * ROWS, p.h + (at + t0 - 1) * p.C, t0, p.C, 1, p.C);
+            me.copy(to, p.f + (at + t0) * p.ld + me.c0, t0, p.ld, 0, p.C);
+            me.copy(to + ROWS, p.v + (at + t0) * p.ld + me.c0, t0, p.ld, 0, p.C);
+            if (p.dh) me.copy(to + 2 * ROWS, p.dh + (at + t0) * p.C + me.c0, t0, p.C, 0, p.C);
+            me.copy(to + 3 * ROWS, p.h + (at + t0 - 1) * p.C + me.c0, t0, p.C, 1, p.C);
         }
         copies_commit();
     };
@@ -409,7 +437,9 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
         copies_wait();
         __syncwarp();
         request(t0 - (STAGES - 1) * me.piece, stage == 0 ? STAGES - 1 : stage - 1);
-        const float *from = mine + stage * W * 4 * ROWS + own * TILE + 2 * me.col;
+        const float *from = Me::row(mine + stage * W * 4 * ROWS, own);
+        const float *pf = p.f + (at + t0 + own) * p.ld + me.c0, *pv = p.v + (at + t0 + own) * p.ld + me.c0;
+        const float *pd = p.dh + (at + t0 + own) * p.C + me.c0, *ph = p.h + (at + t0 + own - 1) * p.C + me.c0;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         Two s[L], e[L], w[L];                               // gate, dh, h[t-1] - v[t]
         Run run = no_steps();
@@ -419,12 +449,11 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
                 const int t = t0 + own + i;
                 s[i] = both(HOLD); e[i] = both(0.f); w[i] = both(0.f);
                 if (all || (t >= 0 && t < me.len)) {
-                    const float *row = from + i * TILE;
-                    Two h = *reinterpret_cast<const Two *>(row + 3 * ROWS);
+                    Two h = me.get(from + 3 * ROWS, i, Me::shift(ph + i * (long long)p.C));
                     if (!all && t == 0) h = h0;
-                    s[i] = sigmoid_less2(*reinterpret_cast<const Two *>(row));
-                    w[i] = less2(h, *reinterpret_cast<const Two *>(row + ROWS));
-                    if (p.dh) e[i] = *reinterpret_cast<const Two *>(row + 2 * ROWS);
+                    s[i] = sigmoid_less2(me.get(from, i, Me::shift(pf + i * p.ld)));
+                    w[i] = less2(h, me.get(from + ROWS, i, Me::shift(pv + i * p.ld)));
+                    if (p.dh) e[i] = me.get(from + 2 * ROWS, i, Me::shift(pd + i * (long long)p.C));
                     const bool kx = keeps(s[i].x), ky = keeps(s[i].y);
                     const Two g = add2(e[i], run.b), ns = Two{-s[i].x, -s[i].y};
                     run.b = fma2(ns, g, pick(kx, ky, g, both(0.f)));
@@ -453,8 +482,8 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
                     x = pick(kx, ky, z, y);
                     Two dv = pick(kx, ky, y, z), df = mul2(mul2(less2(both(1.f), as), y), w[i]);
                     if (!all && t >= me.len) dv = df = both(0.f);
-                    me.template put<BYTES == 16>(pf, df);
-                    me.template put<BYTES == 16>(pv, dv);
+                    me.put(pf, df);
+                    me.put(pv, dv);
                 }
             };
             if (t1 >= 0 && t1 + L <= me.len) write(true);
@@ -468,10 +497,10 @@ template <int W, int L, int BYTES> __global__ void __launch_bounds__(W * 32, 16 
 struct Resident { int clusters[MAX_RANKS + 1]; };
 // Blocks of a cluster: every cluster works through its tile's pieces one after the other, and the clusters that are not resident at once follow in
 // further rounds; the fewest pieces in a row win, and of equal sizes the smallest.  One sequence of 65536 steps and 512 channels, 16 tiles: 13 blocks take
-// 111 us, 8 take 151, and 16, of which 14 clusters are resident, 145.
-template <int W, class P> int launch_scan(void (*kernel)(P), Resident &known, P p, int steps, int tensors, const char *name) {
+// 93 us; with every warp taking part in the exchange 13 took 111, 8 took 151, and 16, of which 14 clusters are resident, 145.
+template <int W, class P> int launch_scan(void (*kernel)(P), Resident &known, P p, int steps, int rows, const char *name) {
     const long long tiles = (long long)p.N * ((p.C + TILE - 1) / TILE);
-    const size_t smem = (size_t)STAGES * W * tensors * steps * TILE * sizeof(float);
+    const size_t smem = (size_t)STAGES * W * rows * sizeof(float);
     if (int s = check_cuda(allow_smem((const void *)kernel, smem), name)) return s;
     // (more than 8 is not promised on every device)
     if (!known.clusters[1]) {
@@ -539,8 +568,8 @@ int seera_gated_scan_fwd(const float *gate, const float *cand, int ld, const flo
     }
     const bool wide = C % 4 == 0 && ld % 4 == 0 && on16({gate, cand}) && on8({h});
     static Resident known[2];
-    if (wide) return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, 16>, known[1], p, 2 * FWD_STEPS, 2, "gated_scan_fwd");
-    return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, 4>, known[0], p, 2 * FWD_STEPS, 2, "gated_scan_fwd");
+    if (wide) return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, true>, known[1], p, 2 * FWD_STEPS, 2 * Place<WARPS, FWD_STEPS, true>::ROWS, "gated_scan_fwd");
+    return launch_scan<WARPS>(scan_fwd_kernel<WARPS, FWD_STEPS, false>, known[0], p, 2 * FWD_STEPS, 2 * Place<WARPS, FWD_STEPS, false>::ROWS, "gated_scan_fwd");
 }
 
 int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const float *h0, const int *lengths, const float *h, const float *dh,
@@ -559,8 +588,8 @@ int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const flo
     }
     const bool wide = C % 4 == 0 && ld % 4 == 0 && ld_grad % 2 == 0 && on16({gate, cand, h, dh}) && on8({dgate, dcand});
     static Resident known[2];
-    if (wide) return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, 16>, known[1], p, 2 * BWD_STEPS, 4, "gated_scan_bwd");
-    return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, 4>, known[0], p, 2 * BWD_STEPS, 4, "gated_scan_bwd");
+    if (wide) return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, true>, known[1], p, 2 * BWD_STEPS, 4 * Place<WARPS, BWD_STEPS, true>::ROWS, "gated_scan_bwd");
+    return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, false>, known[0], p, 2 * BWD_STEPS, 4 * Place<WARPS, BWD_STEPS, false>::ROWS, "gated_scan_bwd");
 }
 
 }  // extern "C"

@@ -429,7 +429,7 @@ struct ResidualBwd {
     long long ld_gate, ld_dgate;
     int rows, C, kind, act, kind2;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 576 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, G == 160 ? 3 : 512 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
     __shared__ Sums sm;
     extern __shared__ __align__(16) float mem[];           // rows on their way, then (or instead) [rows side by side][dgamma, dscale, dgamma2, dbeta2][C],
     typedef Ahead<G, K, V, 5> Rows;                        // the last two with dy
