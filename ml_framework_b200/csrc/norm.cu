@@ -561,30 +561,42 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
 
 // The blocks' sums added up in a fixed order, each of the up to four results to a place of its own (null: not wanted).
 struct ParamSums { float *out[4]; };
-__global__ void __launch_bounds__(1024) param_sums_kernel(const float *__restrict__ partial, const __grid_constant__ ParamSums to, int C, int n, int blocks) {
+// A block has 32 columns; its warps take the rows, V at a time in pieces of V columns a lane.  Measured: 296 blocks' sums of 8192 columns 7.1 us.
+template <int V> __global__ void __launch_bounds__(1024) param_sums_kernel(const float *__restrict__ partial, const __grid_constant__ ParamSums to, int C, int n,
+                                                                           int blocks) {
+    constexpr int ACROSS = 32 / V, AT_ONCE = 4;
     __shared__ float sm[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, c = blockIdx.x * 32 + lane;
-    float t = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, c = blockIdx.x * 32 + lane % ACROSS * V, step = warps * V;
+    Piece<V> t = {};
     if (c < n)
-        for (int s = warp; s < blocks; s += 8 * warps) {
-            float v[8];
+        for (int s = warp * V + lane / ACROSS; s < blocks; s += AT_ONCE * step) {
+            Piece<V> v[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = s + k * warps < blocks ? __ldg(partial + (size_t)(s + k * warps) * n + c) : 0.f;
+            for (int k = 0; k < AT_ONCE; k++) v[k] = s + k * step < blocks ? load<V>(partial + (size_t)(s + k * step) * n + c) : Piece<V>{};
 #pragma unroll
-            for (int k = 0; k < 8; k++) t += v[k];
+            for (int k = 0; k < AT_ONCE; k++)
+#pragma unroll
+                for (int j = 0; j < V; j++) t.x[j] += v[k].x[j];
         }
-    sm[warp][lane] = t;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+#pragma unroll
+        for (int o = ACROSS; o < 32; o <<= 1) t.x[j] += __shfl_xor_sync(0xffffffffu, t.x[j], o);
+        if (lane < ACROSS) sm[warp][lane * V + j] = t.x[j];
+    }
     __syncthreads();
-    if (warp == 0 && c < n) {
-        float r = sm[0][lane];
-        for (int w = 1; w < warps; w++) r += sm[w][lane];
-        float *out = to.out[c / C];
-        if (out) out[c % C] = r;
+    for (int k = warp; k < 32; k += warps) {               // a warp adds up a column
+        float r = lane < warps ? sm[lane][k] : 0.f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+        const int at = blockIdx.x * 32 + k;
+        if (lane == 0 && at < n && to.out[at / C]) to.out[at / C][at % C] = r;
     }
 }
 int param_sums(const float *partial, const ParamSums &to, int C, int sums, int blocks, const char *name) {
     const int n = sums * C, threads = blocks <= 64 ? 256 : (blocks <= 128 ? 512 : 1024);
-    param_sums_kernel<<<(n + 31) / 32, threads, 0, rt().stream>>>(partial, to, C, n, blocks);
+    if (n % 4 == 0) param_sums_kernel<4><<<(n + 31) / 32, threads, 0, rt().stream>>>(partial, to, C, n, blocks);
+    else param_sums_kernel<1><<<(n + 31) / 32, threads, 0, rt().stream>>>(partial, to, C, n, blocks);
     SEERA_LAUNCH_CHECK(name);
     return SEERA_OK;
 }
