@@ -124,8 +124,8 @@ int         seera_get_precision(void);
  *   "tile_n_cap2" / "tile_n_cap3" (64, 128 or 256; defaults 128 / 128): widest accumulator tile used with two /
  *       three bf16 copies per operand; wider tiles raise the arithmetic per byte loaded but leave fewer stages. */
 int         seera_set_option(const char *name, int value);
-/* Status word of the tensor-core kernels: 0 when every bounded wait inside them completed, otherwise
- * the code of the first wait that ran out (1 producer, 2 MMA issuer, 3 epilogue); reading clears it.
+/* Status word of the tensor-core kernels and of the gated scan's clusters: 0 when every bounded wait inside them completed, otherwise
+ * the code of the first wait that ran out (1 producer, 2 MMA issuer, 3 epilogue, 5 a block of a cluster); reading clears it.
  * Synchronises the stream.  -1 if it could not be read. */
 int         seera_tc_device_status(void);
 

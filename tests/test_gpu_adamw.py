@@ -169,3 +169,23 @@ def test_what_is_not_finite(D):
         for q in (pm, pv):
             a = d.down(q, (n,))
             assert np.isnan(a[64:128]).all() and np.isnan(np.delete(a[192:256], 8)).all() and a[200] == np.inf and np.isfinite(a[~block]).all()
+
+
+def test_refusals(D):
+    """Bad arguments are errors of the host: nothing is launched and nothing written."""
+    Dev, capi = D
+    n = 100
+    w = np.arange(n, dtype=np.float32)
+    with Dev() as d:
+        pw, pg, st = d.up(w), d.up(w), d.up(np.zeros(2 * 136, np.uint8), np.uint8)
+        one = lambda q: arr([q], ctypes.c_void_p)  # noqa: E731
+        call = lambda w, g, s, k, step, first: d.L.seera_adamw8_step(1, one(w), one(g), one(s), arr([k], ctypes.c_longlong),  # noqa: E731
+                                                                     arr([0.1], ctypes.c_float), *HP, step, None, first)
+        launches = d.L.seera_launch_count()
+        for bad in ((None, pg, st, n, 1.0, 0), (pw, None, st, n, 1.0, 0), (pw, pg, None, n, 1.0, 0), (pw, pg, st + 4, n, 1.0, 0), (pw, pg, st, -1, 1.0, 0),
+                    (pw, pg, st, n, -1.0, 0), (pw, pg, st, n, float("nan"), 0), (pw, pg, st, n, 1.0, -64), (pw, pg, st, n, 1.0, 32), (pw, pg, st, (1 << 40) + 1, 1.0, 0)):
+            assert call(*bad) != 0
+        assert d.L.seera_adamw8_read(st, pw, None, n) != 0 and d.L.seera_adamw8_read(st + 4, pw, pg, n) != 0 and d.L.seera_adamw8_read(st, pw, pg, -1) != 0
+        assert d.L.seera_launch_count() == launches
+        assert np.array_equal(d.down(pw, (n,)), w)
+        assert call(pw, pg, st, 0, 1.0, 0) == 0 and d.L.seera_launch_count() == launches
