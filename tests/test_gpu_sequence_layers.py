@@ -228,3 +228,54 @@ def test_binding_refuses(E):
             sc.adamw8_read(*bad)
     assert sc.launch_count() == launches
     sc.cuda_free(p)
+
+
+def test_long_ragged_sequences_recorded(E):
+    """Sequences long enough for clusters of blocks, with their lengths on the device, an odd width and one of whole vectors: recorded steps, replayed with the
+    lengths of another batch, against eager ones."""
+    S, sc = E
+    from ml_framework_b200.cuTen import cuten
+    sc.set_precision(3)
+    N, T, IN, U = 2, 1500, 20, 36
+    r = np.random.RandomState(6)
+    X = S.Tensor(r.standard_normal((N, T, IN)).astype(np.float32), is_leaf=True)
+    Y = S.Tensor(np.eye(3, dtype=np.float32)[r.randint(0, 3, N)], is_leaf=True)
+    lengths = [np.array(k, np.int32) for k in ([1500, 1203], [17, 0], [1499, 1500], [1, 700])]
+    out = []
+    for recorded in (False, True):
+        np.random.seed(2)
+        layers = [S.Input((T, IN)), S.GatedRecurrence(IN, U)]
+        layers += [S.RMSNorm(U), S.GatedRecurrence(U, U, output_gate=True), S.GatedResidual(U, residual=layers[1]), S.LayerNorm(U),
+                   S.GatedRecurrence(U, 33, return_sequences=False), S.Dense(33, 3, activation="softmax")]
+        model = S.Sequential(layers)
+        opt = S.AdamW(model, lr=1e-3)
+        at = cuten(lengths[0], "int32")
+
+        def step():
+            loss = S.Loss().categorical_cross_entropy(model.forward(X, lengths=at), Y)
+            model.zero_grad()
+            S.autograd4nn(loss)
+            opt.step()
+            return loss
+        step(), step()
+        if recorded:
+            opt._scalars_in_graph = True
+            sc.graph_begin()
+            kept = step()
+            opt._scalars_in_graph = False
+            g = sc.graph_end()
+        for k in range(1, 8):
+            other = cuten(lengths[k % 4], "int32")
+            sc.cuda_memcopy_devicetodevice(at.main_ptr, other.main_ptr, N)
+            if recorded:
+                sc.graph_set_scalars(g, opt._scalars())
+                sc.graph_launch(g)
+            else:
+                step()
+            sc.stream_synchronize()
+        assert sc.tc_device_status() == 0
+        out.append(model.params.to_host_f32().copy())
+        if recorded:
+            sc.graph_destroy(g)
+            del kept
+    assert np.isfinite(out[0]).all() and np.array_equal(out[0], out[1])
