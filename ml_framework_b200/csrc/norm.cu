@@ -376,11 +376,8 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
         }
         in.next();
     };
-    if (Rows::ON)
-        for (int k = 0; k < Rows::STAGES - 1; k++) request(row + k * step);
     for (; row < p.rows; row += step) {
-        request(Rows::ON ? row + (Rows::STAGES - 1) * step : row);
-        in.wait();
+        request(row);
         const long long at = (long long)row * p.C;
         Piece<V> x[K], q[K], r[K];
 #pragma unroll
@@ -630,11 +627,15 @@ template <class Fn> int by_width(int C, bool vec, Fn fn) {
     return vec ? by_threads(C, fn, Int<2>{}, Int<4>{}) : by_threads(C, fn, Int<8>{}, Int<1>{});
 }
 // Blocks of a launch that keeps sums over the rows: as many as are resident at once, so that each writes its sums once.
-int resident_grid(const void *kernel, int threads, size_t smem, int rows, int rows_at_once, int *grid) {
-    int per_sm = 0;
-    if (int s = check_cuda(allow_smem(kernel, smem), "norm: shared memory")) return s;
-    if (int s = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem), "norm: occupancy")) return s;
-    const long long need = ((long long)rows + rows_at_once - 1) / rows_at_once, most = (long long)rt().sm_count * (per_sm > 0 ? per_sm : 1);
+// (`known` is the kernel's: asking takes the host longer than half a launch.)
+struct PerSm { size_t smem = 0; int blocks = 0; };
+int resident_grid(PerSm &known, const void *kernel, int threads, size_t smem, int rows, int rows_at_once, int *grid) {
+    if (!known.blocks || known.smem != smem) {
+        if (int s = check_cuda(allow_smem(kernel, smem), "norm: shared memory")) return s;
+        if (int s = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known.blocks, kernel, threads, smem), "norm: occupancy")) return s;
+        known.smem = smem;
+    }
+    const long long need = ((long long)rows + rows_at_once - 1) / rows_at_once, most = (long long)rt().sm_count * (known.blocks > 0 ? known.blocks : 1);
     *grid = (int)(need < most ? need : most);
     return SEERA_OK;
 }
@@ -663,7 +664,8 @@ int seera_norm_fwd(const float *x, const float *gamma, const float *beta, float 
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
         const size_t smem = ROWS_OF<G> * Ahead<G, K, V, 1>::FLOATS * sizeof(float);
         int grid = (int)(((long long)rows + ROWS_OF<G> - 1) / ROWS_OF<G>);
-        if (Ahead<G, K, V, 1>::ON) if (int s = resident_grid((const void *)norm_fwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
+        static PerSm known;
+        if (Ahead<G, K, V, 1>::ON) if (int s = resident_grid(known, (const void *)norm_fwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
         norm_fwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("norm_fwd");
         return (int)SEERA_OK;
@@ -681,7 +683,8 @@ int seera_norm_bwd(const float *dy, const float *x, const float *gamma, const fl
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
         const size_t smem = ROWS_OF<G> * std::max(Ahead<G, K, V, 2>::FLOATS, (size_t)2 * C) * sizeof(float);
         int grid;
-        if (int s = resident_grid((const void *)norm_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
+        static PerSm known;
+        if (int s = resident_grid(known, (const void *)norm_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
         float *partial = (float *)scratch_alloc((size_t)grid * 2 * C * sizeof(float));
         if (!partial) return (int)SEERA_E_OOM;
         const NormBwd p{dy, x, gamma, stats, dx, partial, rows, C, kind};
@@ -709,10 +712,8 @@ int seera_gated_residual_fwd(const float *u, const float *gate, int ld_gate, con
     const bool vec = C % 4 == 0 && (!gate || ld_gate % 4 == 0) && all16({u, gate, res, gamma, res ? scale : nullptr, out, y, y ? next_gamma : nullptr, y ? next_beta : nullptr});
     return by_width(C, vec, [&](auto g_, auto k_, auto v_) {
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
-        const size_t smem = ROWS_OF<G> * Ahead<G, K, V, 3>::FLOATS * sizeof(float);
-        int grid = (int)(((long long)rows + ROWS_OF<G> - 1) / ROWS_OF<G>);
-        if (Ahead<G, K, V, 3>::ON) if (int s = resident_grid((const void *)residual_fwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
-        residual_fwd_kernel<G, K, V><<<grid, THREADS_OF<G>, smem, rt().stream>>>(p);
+        const int grid = (int)(((long long)rows + ROWS_OF<G> - 1) / ROWS_OF<G>);
+        residual_fwd_kernel<G, K, V><<<grid, THREADS_OF<G>, 0, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("gated_residual_fwd");
         return (int)SEERA_OK;
     });
@@ -737,7 +738,8 @@ int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u,
         constexpr int G = decltype(g_)::value, K = decltype(k_)::value, V = decltype(v_)::value;
         const size_t smem = ROWS_OF<G> * std::max(Ahead<G, K, V, 5>::FLOATS, (size_t)sums * C) * sizeof(float);
         int grid;
-        if (int s = resident_grid((const void *)residual_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
+        static PerSm known;
+        if (int s = resident_grid(known, (const void *)residual_bwd_kernel<G, K, V>, THREADS_OF<G>, smem, rows, ROWS_OF<G>, &grid)) return s;
         float *partial = (float *)scratch_alloc((size_t)grid * sums * C * sizeof(float));
         if (!partial) return (int)SEERA_E_OOM;
         const ResidualBwd p{dout, dy, u, gate, res, gamma, scale, next_gamma, stats, du, dgate, dres, partial, ld_gate, ld_dgate, rows, C, kind, act, next_kind};
