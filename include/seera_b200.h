@@ -533,7 +533,8 @@ int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u,
  * seera_adamw8_step holds m and v in 8 bits: `state` of a tensor is seera_adamw8_state_bytes(n) bytes (8-byte aligned; zeros to start
  * with), 136 for each 64 neighbouring entries: sixteen times four codes of m and four of v, then the largest |m| and the largest v of the 64 as
  * floats.  A code times the block's largest is the entry: m has a sign, 4 bits of exponent and 3 of mantissa, v 5 bits of exponent and 3 of mantissa.
- * Rounding goes up or down at random with the value as its mean; the random bits follow from `step` (the number of the step, a whole number below 2^24)
+ * Rounding goes up or down at random with the value as its mean, but a v above zero never to 0 (2^-33 of its block's largest at least: the m beside it may
+ * have been rounded up to 2^-17 of the largest, and m / sqrt(v) has no other bound); the random bits follow from `step` (the number of the step, a whole number below 2^24)
  * and the entry's place: `first`, a multiple of 64, plus its place in the tensors one after the other, each rounded up to 64.  w is updated from
  * m and v before they are rounded.  An infinity or a NaN in a gradient leaves none of the m and v of its 64 entries finite, where 32 bits would keep it to the one.
  * seera_adamw8_read writes out the m and v that a state of n entries stands for. */

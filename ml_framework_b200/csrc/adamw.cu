@@ -18,6 +18,9 @@
 // Rounding goes up with the probability of the distance gone, from 16 random bits each: the code's mean is the value.  Rounded to nearest, v would
 // stand still: beta2 = 0.999 moves it by at most 0.1 % of itself a step where half a code is 3 to 6 %.  The random bits are a hash of the
 // entry's place and the step, so a step is reproducible.  The weights are updated from the averages as they are before rounding.
+// A v above zero takes the smallest code at least.  At 0, beside an m that was rounded up to 2^-17 of its block's largest, the next step would divide that m by
+// the root of the newest gradient alone: entries 2^-17 below their block's largest went up to 1000 lr in a step.  The smallest v has a root of 2^-16.5, the smallest
+// m is 2^-17: what lies below both goes in steps that are too small (of 2^-20 a quarter to a half of what 32 bits do), and none is much larger than theirs.
 #include "common.cuh"
 #include "internal.h"
 #include "pairs.cuh"
@@ -227,6 +230,7 @@ __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__
     }
     float im, iv;
     const float lm = held(am, im), lv = held(av, iv);
+    const unsigned least = lv > 0.f && lv < __int_as_float(0x7f800000) ? 1u << 20 : 0u;         // the smallest code of v in its place
     const unsigned seed = random_seed((unsigned long long)(t.place + at + i), (unsigned)a.step);
     unsigned qm[8], qv[8];
 #pragma unroll
@@ -234,7 +238,8 @@ __global__ void __launch_bounds__(THREADS) adamw8_kernel(const __grid_constant__
         const unsigned r0 = random32(seed ^ (2 * j)), r1 = random32(seed ^ (2 * j + 1));
         const Two sm = scaled(m[j], im, M_UNIT), sv = scaled(v[j], iv, V_UNIT);
         qm[2 * j] = rounded(sm.x, r0 & 0xffffu); qm[2 * j + 1] = rounded(sm.y, r1 & 0xffffu);
-        qv[2 * j] = rounded(sv.x, r0 >> 16); qv[2 * j + 1] = rounded(sv.y, r1 >> 16);
+        qv[2 * j] = max(rounded(sv.x, r0 >> 16), v[j].x > 0.f ? least : 0u);
+        qv[2 * j + 1] = max(rounded(sv.y, r1 >> 16), v[j].y > 0.f ? least : 0u);
     }
     if (there) {
 #pragma unroll
