@@ -1106,7 +1106,8 @@ class GatedRecurrence(_ParamLayer):
             if initializer not in table:
                 raise ValueError(f"Initializer must be one of {list(table.keys())}")
         self.in_units, self.units, self.output_gate = int(in_units), int(units), bool(output_gate)
-        self.return_sequences, self.stateful, self.training, self._state = bool(return_sequences), bool(stateful), True, None
+        self.return_sequences, self.stateful, self.training = bool(return_sequences), bool(stateful), True
+        self._state, self._started, self._recorded = None, False, {}
         self._cols = (3 if output_gate else 2) * self.units
         self._w_init = _initial(table[kernel_initializer], (self.in_units, self._cols))
         self._b_init = _initial(table[bias_initializer], (1, self._cols))
@@ -1114,8 +1115,28 @@ class GatedRecurrence(_ParamLayer):
         self.bais = Tensor(self._b_init, is_leaf=True)
 
     def reset_states(self):
-        """The next `predict` starts from zeros again."""
-        self._state = None
+        """The next `predict` starts from zeros again, with as many sequences as it likes; a recording's next replay too."""
+        self._started = False
+        states = list(self._recorded.values())
+        for s in states if self._state is None or self._state in states else states + [self._state]:
+            sc.cuda_memset(s.main_ptr, 0, 4 * s.size)       # in place: a recording goes on from the tensor that it was made with
+
+    def _state_of(self, N):
+        """The state that a prediction of N sequences goes on from.  What a recording has gone on from stays as long as the layer."""
+        s = self._state
+        if s is None or (s.shape[0] != N and not self._started):
+            s = self._recorded.get(N)
+            if s is None:
+                if sc.is_capturing():
+                    raise RuntimeError("a recording goes on from a state: predict once before it")
+                s = _wrap(sc.cuda_zeros_f(N * self.units), (N, self.units))
+            self._state = s
+        if s.shape[0] != N:
+            raise ValueError(f"the state is that of {s.shape[0]} sequences, the input has {N}: reset_states() first")
+        if sc.is_capturing():
+            self._recorded[N] = s
+        self._started = True
+        return s
 
     def forward(self):
         x = self.inputs = self.inpobj.outputs
@@ -1130,15 +1151,7 @@ class GatedRecurrence(_ParamLayer):
         lengths = model._lengths if model is not None else None
         if lengths is not None and lengths.size != N:
             raise ValueError(f"{lengths.size} lengths for {N} sequences")
-        state = None
-        if self.stateful and not self.training:
-            if self._state is None:
-                if sc.is_capturing():
-                    raise RuntimeError("a recording goes on from a state: predict once before it")
-                self._state = _wrap(sc.cuda_zeros_f(N * U), (N, U))
-            state = self._state
-            if state.shape != (N, U):
-                raise ValueError(f"the state is that of {state.shape[0]} sequences, the input has {N}: reset_states() first")
+        state = self._state_of(N) if self.stateful and not self.training else None
         z = _new((N, T, cols))
         ha, hw, _ = sc.matmul_bias_act_fwd_s(xv.main_ptr, wv.main_ptr, b.value.main_ptr, z._ptr, M, cols, K, 0, 0, False)
         kept_a, kept_w = _KeptRows(ha) if ha else None, _KeptRows(hw) if hw else None
