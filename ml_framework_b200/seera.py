@@ -99,6 +99,9 @@ class Tensor:
     _rows = None                     # row-major copies of the value, made by its producer for a Dense layer
     _pass = None                     # (input shape, reference to the model) of the pass it came from
     _gate = None                     # a GatedRecurrence's output: the _OutputGate beside it
+    _copies_grad = False             # its backward makes the gradient's 16-bit copies (fp16 modes: under the factor in force)
+    _resizes_grad = False            # its backward's gradients may be larger or smaller than its own by any factor
+    _sets_factor = False             # its backward takes the factor anew, from a gradient of its own
 
     def __init__(self, value, dtype="float32", is_leaf=False, device="cuda"):
         if isinstance(value, Tensor):
@@ -400,12 +403,41 @@ class autograd4nn:
             if not t.is_leaf:
                 t.grad = None
         self.hook.grad = cuten.ones_like(self.hook.value)
+        factor = None
+        if sc.get_precision() in (4, 5) and any(t._resizes_grad or t._sets_factor for t in order):
+            factor = _Factor(order, self.hook)
         for t in reversed(order):
             back, g = t._backward, t.grad
             if back is not None and g is not None:
                 if g.__class__ is _PooledGrad and not t._takes_pooled:
                     t.grad = g = g.materialize()
+                if factor is not None:
+                    factor.for_gradient(t, g)
                 back(g)
+
+
+class _Factor:
+    """The factor of the fp16 modes' gradient copies in a pass through layers that may change a gradient's size by any factor (a norm divides by its row's
+    size; the residual of a GatedResidual goes past what its branch divides by).  There is one factor at a time.  The loss sets it, and it holds for a gradient
+    that came from there through layers that keep the size, alone: not for a sum of several, and no longer once it has been set for another.  Where
+    copies are made of a gradient that it does not hold for it is taken anew, from that gradient."""
+    __slots__ = ("holds", "uses")
+
+    def __init__(self, order, hook):
+        self.holds, self.uses = {hook}, {}
+        for t in order:
+            for p in t._parents:
+                self.uses[p] = self.uses.get(p, 0) + 1
+
+    def for_gradient(self, t, g):
+        """Before t's backward is called with its gradient g."""
+        if t._sets_factor:
+            self.holds = {t}
+        elif t._copies_grad and t not in self.holds:
+            _rescale_gradients(g.gp if g.__class__ is _PooledGrad else g)
+            self.holds = {t}
+        if t in self.holds and not t._resizes_grad:
+            self.holds.update(p for p in t._parents if self.uses[p] == 1)
 
 
 # ─────────────────────────────────────────────────────────────────────────────────────────────
@@ -509,6 +541,7 @@ class _ParamLayer(Layer):
         """The layer's output Tensor around `z`, which holds act(contraction + bias), or the logits of a softmax (`softmax`, where its values
         came with them)."""
         node = Tensor._of(z, (x, self.weights, self.bais), node_backward)
+        node._copies_grad = True
         if takes_pooled:
             node._takes_pooled = True
         if self.layeract != "softmax":
@@ -1006,8 +1039,7 @@ _GATES = {None: 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4}
 
 
 def _rescale_gradients(g):
-    """Behind a layer whose gradient may be larger than the loss's by any factor (a norm divides by its row's size) the fp16 precision modes
-    take the factor of their gradient copies anew."""
+    """The fp16 precision modes take the factor of their gradient copies anew, from g."""
     if sc.get_precision() in (4, 5):
         sc.grad_scale_update(g.main_ptr, g.size)
 
@@ -1051,6 +1083,7 @@ class _FeatureNorm(_ParamLayer):
             self.inpobj._normed = None
             owner = self._model
             self.outputs = out = Tensor._of(made[1], (x, g, b), lambda dy: x._accumulate(_NormGrad(dy, (g, b, owner))))
+            out._resizes_grad = True
             return out
         y, stats = _new(shape), _new((rows, 2))
         sc.norm_fwd(xv.main_ptr, g.value.main_ptr, b.value.main_ptr, y._ptr, stats._ptr, rows, C, kind, self.eps)
@@ -1060,10 +1093,9 @@ class _FeatureNorm(_ParamLayer):
             dg, db = g._grad_target(), b._grad_target()
             dx = _new(shape) if need_dx else None
             sc.norm_bwd(dy.main_ptr, xv.main_ptr, g.value._ptr, stats._ptr, dx._ptr if need_dx else 0, dg._ptr, db._ptr, rows, C, kind)
-            if need_dx:
-                _rescale_gradients(dx)
             _deliver(owner, x, g, b, dx, dg, db)
         self.outputs = out = Tensor._of(y, (x, g, b), backward)
+        out._resizes_grad = True
         return out
 
     def __repr__(self):
@@ -1188,7 +1220,7 @@ class GatedRecurrence(_ParamLayer):
                     k.release()
             _deliver(owner, x, W, b, dx, dw, db)
         self.outputs = out = Tensor._of(h if whole else last, (x, W, b), backward)
-        out._gate = gate
+        out._gate, out._sets_factor = gate, True
         return out
 
     def __repr__(self):
@@ -1264,8 +1296,6 @@ class GatedResidual(_ParamLayer):
                                   rows, C, kind, act, kind2)
             if rv is None:
                 sc.cuda_memset(db.main_ptr, 0, 4 * C)
-            if need_du:
-                _rescale_gradients(du)
             if dy is not None:
                 _deliver(nowner, None, ng, nb, None, dng, dnb)
             if need_dr:
@@ -1273,6 +1303,7 @@ class GatedResidual(_ParamLayer):
             _deliver(owner, u, g, b, du if not u.is_leaf else None, dg, db)
         parents = (u, g, b) if r is None else (u, r, g, b)
         self.outputs = t = Tensor._of(out, parents, backward)
+        t._resizes_grad = True
         return t
 
     def __repr__(self):
