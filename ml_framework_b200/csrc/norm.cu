@@ -118,15 +118,16 @@ template <int K, int V> __device__ __forceinline__ void gate_slopes(Piece<V> (&g
     }
 }
 
-// The rows of N tensors on their way to the thread that works on them, STAGES - 1 rows ahead: each thread copies what it will read itself, so that
+// The rows of N tensors on their way to the thread that works on them, one row ahead: each thread copies what it will read itself, so that
 // nothing has to be waited for but its own copies, and the loads hold no registers.  Rows of more than 8 floats a thread would not leave room for it.
-// (A place of its own for each thread, at constant distances, took 331 us where the copies of a warp side by side take 222.)
-// With three tensors, the forward of the residual, loads into registers by twice the blocks are faster (16384 x 2048: 117 against 133 us), with
-// one 70 against 55, with two 108 against 83, with five 245 against 222.
+// (A place of its own for each thread, at constant distances, took half as long again as the copies of a warp side by side.)
+// Loads into registers instead, us of 16384 x 2048 / 2047: with one tensor 53 / 64 (here 51 / 75), with two 102 / 109 (77 / 103), with five 222 / 367 (203 / 313).
+// With three, the forward of the residual, they are used: 113 / 141 (a row ahead: 115 / 209, the odd row's single copies and reads).
+// Two rows ahead: 52, 81 and, with half the blocks, 300 us of 2048.
 template <int K, int V> constexpr bool AHEAD = K * V <= 8;
 template <int G, int K, int V, int N> struct Ahead {
     static constexpr bool ON = AHEAD<K, V> && N != 3;
-    static constexpr int STAGES = N > 2 ? 2 : 3;
+    static constexpr int STAGES = 2;
     static constexpr int STAGE = N * K * V * G;
     static constexpr size_t FLOATS = ON ? STAGES * STAGE : 0;          // of a row
     float *mine, *asked;                                   // asked: the stage that is asked for next
@@ -154,8 +155,9 @@ template <int G, int K, int V, int N> struct Ahead {
         asm volatile("cp.async.commit_group;" ::: "memory");
         asked = asked + STAGE == mine + STAGES * STAGE ? mine : asked + STAGE;
     }
-    // The row that was asked for STAGES - 1 calls of `next()` ago is there, in the stage that is asked for next.
-    __device__ __forceinline__ void wait() { if (ON) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+    // The row that was asked for in front of the last STAGES - 1 calls of `next()` is there, in the stage that is asked for next; those asked for since may
+    // still be on their way.
+    __device__ __forceinline__ void wait() { if (ON) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
     __device__ __forceinline__ Piece<V> take(int i, int k, bool there) const {
         if constexpr (ON) return there && (t + k * G) * V < C ? load<V>(place(i, k)) : Piece<V>{};
         else return now[i][k];
@@ -435,7 +437,7 @@ struct ResidualBwd {
     long long ld_gate, ld_dgate;
     int rows, C, kind, act, kind2;
 };
-template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, G == 160 ? 3 : 512 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
+template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 512 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
     __shared__ Sums sm;
     extern __shared__ __align__(16) float mem[];           // rows on their way, then (or instead) [rows side by side][dgamma, dscale, dgamma2, dbeta2][C],
     typedef Ahead<G, K, V, 5> Rows;                        // the last two with dy
