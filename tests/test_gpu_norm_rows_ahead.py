@@ -6,7 +6,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 # every width of a block, whole vectors and single words; enough rows for more than four a block of any of them (at most 16 blocks of 8 rows or 32 of one an SM)
-WIDTHS = [(64, 80000), (255, 80000), (500, 20000), (513, 20000), (1000, 20000), (1279, 10000), (1280, 10000), (1536, 10000), (2047, 8000), (2048, 8000), (4095, 6000),
+WIDTHS = [(64, 80000), (255, 80000), (500, 20000), (513, 20000), (767, 20000), (768, 20000), (1000, 20000), (1279, 10000), (1280, 10000), (1536, 10000), (2047, 8000), (2048, 8000), (2559, 6000), (2560, 6000), (3300, 6000), (4095, 6000),
           (4096, 6000)]
 
 
