@@ -37,8 +37,9 @@ template <int V> struct Piece { float x[V]; };
 template <int V> __device__ __forceinline__ Piece<V> load(const float *p);
 template <> __device__ __forceinline__ Piece<4> load<4>(const float *p) { const float4 v = *reinterpret_cast<const float4 *>(p); return {v.x, v.y, v.z, v.w}; }
 template <> __device__ __forceinline__ Piece<1> load<1>(const float *p) { return {*p}; }
-// Zeros behind a row's end.  The backward kernels on single words go through all of a thread's pieces, so that the loads of one do not wait for whether
-// another is there (16384 x 2047: 339 us against 409); with V = 4, and in the forward kernels, ending early is faster (208 against 218, 154 against 186).
+// Zeros behind a row's end.  Kernels that do not end at it go through all of a thread's pieces, so that the loads of one do not wait for whether another is
+// there.  Measured at 16384 rows: norm backward, single words 104 us of 2047 (ending early 109), V = 4 54 of 1280 when it ends early (60 when not); residual backward, single words
+// 313 of 2047 (393), V = 4 see ENDS; the forward kernels end early (154 against 186 us).
 template <int V> __device__ __forceinline__ Piece<V> load_if(const float *p, bool there) { return there ? load<V>(p) : Piece<V>{}; }
 template <int V> __device__ __forceinline__ void store(float *p, const Piece<V> &v);
 template <> __device__ __forceinline__ void store<4>(float *p, const Piece<4> &v) { *reinterpret_cast<float4 *>(p) = make_float4(v.x[0], v.x[1], v.x[2], v.x[3]); }
@@ -438,6 +439,9 @@ struct ResidualBwd {
     int rows, C, kind, act, kind2;
 };
 template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 512 / THREADS_OF<G>) residual_bwd_kernel(const __grid_constant__ ResidualBwd p) {
+    // Whether pieces behind a row's end are left out.  Going through them is faster where registers allow (16384 x 2048 194 against 203 us, x 1280 128 against 136,
+    // x 768 82 against 85), not for rows of a warp (65536 x 256 104 against 99) and where it spills (8192 x 4096 271 against 231, x 3300 259 against 237).
+    constexpr bool ENDS = V > 1 && (G == 32 || G > 320);
     __shared__ Sums sm;
     extern __shared__ __align__(16) float mem[];           // rows on their way, then (or instead) [rows side by side][dgamma, dscale, dgamma2, dbeta2][C],
     typedef Ahead<G, K, V, 5> Rows;                        // the last two with dy
@@ -489,10 +493,10 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
             for (int k = 0; k < K; k++) {
                 const int c = (t + k * G) * V;
                 e[k] = in.take(4, k, true);
-                if (V > 1 && c >= p.C) break;
-                const Piece<V> ga = load_if<V>(p.gamma + c, V > 1 || c < p.C), g2 = load_if<V>(p.gamma2 + c, V > 1 || c < p.C);
+                if (ENDS && c >= p.C) break;
+                const Piece<V> ga = load_if<V>(p.gamma + c, ENDS || c < p.C), g2 = load_if<V>(p.gamma2 + c, ENDS || c < p.C);
                 Piece<V> sc = {}, q[1] = {g[k]};
-                if (p.res) sc = load_if<V>(p.scale + c, V > 1 || c < p.C);
+                if (p.res) sc = load_if<V>(p.scale + c, ENDS || c < p.C);
                 if (!Rows::ON && p.gate) gate_values<1, V>(q, p.act);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
@@ -513,7 +517,7 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
             const float m0 = p.kind2 == SEERA_NORM_LAYER ? s.x * inv : 0.f, m1 = s.y * inv;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                if (V > 1 && (t + k * G) * V >= p.C) break;
+                if (ENDS && (t + k * G) * V >= p.C) break;
 #pragma unroll
                 for (int j = 0; j < V; j++) d[k].x[j] += st.w * (e[k].x[j] - m0 - n2[k].x[j] * m1);
             }
@@ -522,15 +526,15 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int c = (t + k * G) * V;
-            if (V > 1 && c >= p.C) break;
-            const Piece<V> ga = load_if<V>(p.gamma + c, V > 1 || c < p.C);
+            if (ENDS && c >= p.C) break;
+            const Piece<V> ga = load_if<V>(p.gamma + c, ENDS || c < p.C);
             if (p.res) {
-                const Piece<V> sc = load_if<V>(p.scale + c, V > 1 || c < p.C);
+                const Piece<V> sc = load_if<V>(p.scale + c, ENDS || c < p.C);
                 Piece<V> o;
                 sum_scale.add(k, c, [&](int j) { return d[k].x[j] * r[k].x[j]; });
 #pragma unroll
                 for (int j = 0; j < V; j++) o.x[j] = sc.x[j] * d[k].x[j];
-                if (p.dres && (V > 1 || c < p.C)) store<V>(p.dres + at + c, o);
+                if (p.dres && (ENDS || c < p.C)) store<V>(p.dres + at + c, o);
             }
             if (p.gate) {
                 Piece<V> o, q[1] = {g[k]}, sl[1] = {slope[Rows::ON ? k : 0]};
@@ -540,7 +544,7 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
                     o.x[j] = d[k].x[j] * (ga.x[j] * n[k].x[j]) * sl[0].x[j];
                     d[k].x[j] *= q[0].x[j];
                 }
-                if (p.dgate && (V > 1 || c < p.C)) store<V>(p.dgate + row * p.ld_dgate + c, o);
+                if (p.dgate && (ENDS || c < p.C)) store<V>(p.dgate + row * p.ld_dgate + c, o);
             }
             sum_gamma.add(k, c, [&](int j) { return d[k].x[j] * n[k].x[j]; });
 #pragma unroll
@@ -555,7 +559,7 @@ template <int G, int K, int V> __global__ void __launch_bounds__(THREADS_OF<G>, 
         for (int k = 0; k < K; k++) {
             const int c = (t + k * G) * V;
             if (c >= p.C || !p.du) {
-                if (V > 1) break;
+                if (ENDS) break;
                 continue;
             }
             Piece<V> o;
