@@ -499,6 +499,9 @@ int seera_gated_scan_fwd(const float *gate, const float *cand, int ld, const flo
                          int C);
 int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const float *h0, const int *lengths, const float *h, const float *dh,
                          const float *dh_last, float *dgate, float *dcand, int ld_grad, float *dh0, int N, int T, int C);
+/* A padded batch x [N, T, C] with zeros behind each sequence's length (values outside 0..T as above): what is there is not read and may be anything, infinities and
+ * NaNs too, which a product over all steps would carry into its sums.  y may be x. */
+int seera_pad_steps(const float *x, const int *lengths, float *y, int N, int T, int C);
 /* Norms over the C features of each row (C <= 8192, else SEERA_E_LIMIT):  N(x) = (x - mu) / sqrt(mean((x - mu)^2) + eps), with mu the row's
  * mean or, for SEERA_NORM_RMS, 0.
  *     seera_norm_fwd   y = gamma N(x) + beta;  beta may be NULL; stats (rows x 2 floats, for the backward; 8-byte aligned) may be NULL

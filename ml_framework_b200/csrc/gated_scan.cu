@@ -543,6 +543,25 @@ bool on8(std::initializer_list<const void *> ps) {
     for (const void *p : ps) if ((uintptr_t)p & 7) return false;
     return true;
 }
+// A padded batch with zeros behind each sequence's length; what is there is not read.  A sequence's floats in a row, so that a place is behind the length where it is not
+// below length x C: bytes bound it (read and written once).
+template <bool VEC> __global__ void __launch_bounds__(256) pad_steps_kernel(const float *x, const int *__restrict__ lengths, float *y, int N, int T, int C) {
+    constexpr int V = VEC ? 4 : 1;
+    const long long all = (long long)T * C, step = (long long)gridDim.x * 256 * V;
+    for (int n = blockIdx.y; n < N; n += gridDim.y) {
+        const long long live = (long long)length_of(lengths, n, T) * C;
+        const float *from = x + n * all;
+        float *to = y + n * all;
+        for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < all; i += step) {
+            if (VEC && i + V <= live) {
+                *reinterpret_cast<float4 *>(to + i) = *reinterpret_cast<const float4 *>(from + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) to[i + j] = i + j < live ? from[i + j] : 0.f;
+            }
+        }
+    }
+}
 // Few steps: a thread per state has nothing to split.
 constexpr int SERIAL_STEPS = 16;
 }  // namespace
@@ -590,6 +609,22 @@ int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const flo
     static Resident known[2];
     if (wide) return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, true>, known[1], p, 2 * BWD_STEPS, 4 * Place<WARPS, BWD_STEPS, true>::ROWS, "gated_scan_bwd");
     return launch_scan<WARPS>(scan_bwd_kernel<WARPS, BWD_STEPS, false>, known[0], p, 2 * BWD_STEPS, 4 * Place<WARPS, BWD_STEPS, false>::ROWS, "gated_scan_bwd");
+}
+
+int seera_pad_steps(const float *x, const int *lengths, float *y, int N, int T, int C) {
+    SEERA_ENSURE();
+    const long long all = (long long)T * C;
+    if (N < 0 || T < 0 || C < 1 || (N > 0 && T > 0 && (!x || !lengths || !y))) return fail(SEERA_E_ARG, "pad_steps: bad argument");
+    if (N == 0 || T == 0) return SEERA_OK;
+    ProfBytes pb(8.0 * N * all, "pad_steps");
+    const bool wide = all % 4 == 0 && on16({x, y});
+    const int deep = N < 65535 ? N : 65535;
+    const long long need = (all + (wide ? 1023 : 255)) / (wide ? 1024 : 256), most = (long long)rt().sm_count * 8 / deep + 1;
+    const dim3 grid((unsigned)(need < most ? need : most), (unsigned)deep);
+    if (wide) pad_steps_kernel<true><<<grid, 256, 0, rt().stream>>>(x, lengths, y, N, T, C);
+    else pad_steps_kernel<false><<<grid, 256, 0, rt().stream>>>(x, lengths, y, N, T, C);
+    SEERA_LAUNCH_CHECK("pad_steps");
+    return SEERA_OK;
 }
 
 }  // extern "C"

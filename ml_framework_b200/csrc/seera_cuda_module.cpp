@@ -201,6 +201,7 @@ PYBIND11_MODULE(seera_cuda, m) {
     m.def("gated_scan_bwd", [](uptr f, uptr v, int ld, uptr h0, uptr len, uptr h, uptr dh, uptr dlast, uptr df, uptr dv, int ldg, uptr dh0, int N, int T, int C) {
         ck(seera_gated_scan_bwd(P<const F>(f), P<const F>(v), ld, P<const F>(h0), P<const int>(len), P<const F>(h), P<const F>(dh), P<const F>(dlast),
                                 P<F>(df), P<F>(dv), ldg, P<F>(dh0), N, T, C)); });
+    m.def("pad_steps", [](uptr x, uptr len, uptr y, int N, int T, int C) { ck(seera_pad_steps(P<const F>(x), P<const int>(len), P<F>(y), N, T, C)); });
     m.def("norm_fwd", [](uptr x, uptr g, uptr b, uptr y, uptr st, int rows, int C, int kind, float eps) {
         ck(seera_norm_fwd(P<const F>(x), P<const F>(g), P<const F>(b), P<F>(y), P<F>(st), rows, C, kind, eps)); });
     m.def("norm_bwd", [](uptr dy, uptr x, uptr g, uptr st, uptr dx, uptr dg, uptr db, int rows, int C, int kind) {

@@ -474,11 +474,28 @@ class Input(Layer):
         self.inputs = None
 
     def forward(self):
-        self.outputs = self.inputs
-        return self.outputs
+        x, model = self.inputs, self._model and self._model()
+        if model is not None and model._lengths is not None and len(x.value.shape) > 2:
+            x = _padded(x, model._lengths)
+        self.outputs = x
+        return x
 
     def __repr__(self):
         return f"Input Layer with shape {self.shape}"
+
+
+def _padded(x, lengths):
+    """x with zeros behind each sequence's length.  What a caller's batch has there may be anything: layers that do not go through time read every step, and a
+    weight gradient would be NaN from a NaN there times the zero that the step's gradient is."""
+    shape = x.value.shape
+    N, T = shape[:2]
+
+    def pad(v):
+        y = _new(shape)
+        sc.pad_steps(v.main_ptr, lengths.main_ptr, y._ptr, N, T, _numel(shape[2:]))
+        return y
+    y = pad(x.value)
+    return Tensor(y, is_leaf=True) if x.is_leaf else Tensor._of(y, (x,), lambda g: x._accumulate(pad(g)))
 
 
 def _initial(kind_scale, shape):
@@ -1400,7 +1417,7 @@ class Sequential:
         self._passes = set()                          # kinds and sizes of passes made (see _open_batch)
         self._build_arena()
         self._ref = weakref.ref(self)
-        for l in self.param_layers:
+        for l in [self.model[0]] + self.param_layers:
             l._model = self._ref
 
     # one contiguous block each for parameters and gradients; slots are 64-float aligned
@@ -1449,7 +1466,7 @@ class Sequential:
 
     def forward(self, X=None, lengths=None):
         """`lengths`: how many steps each sequence of an (N, T, ...) input has, for the layers that go through time: host integers or a
-        device tensor of int32."""
+        device tensor of int32.  What the input has behind them is not read: it counts as zeros."""
         if X is not None:
             if isinstance(X, np.ndarray):
                 X = Tensor(X, is_leaf=True)

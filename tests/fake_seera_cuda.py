@@ -619,6 +619,12 @@ def gated_scan_bwd(f, v, ld, h0, lengths, h, dh, dlast, df, dv, ldg, dh0, N, T, 
         F(dh0, (N, C))[:] = c
 
 
+def pad_steps(x, lengths, y, N, T, C):
+    _count("pad_steps")
+    live = np.arange(T)[None, :] < _view(lengths, N, np.int32)[:, None]
+    F(y, (N, T, C))[:] = np.where(live[..., None], F(x, (N, T, C)), np.float32(0))
+
+
 _norm_eps = {}
 
 
