@@ -26,6 +26,7 @@
 #include "pairs.cuh"
 #include <cuda_fp16.h>
 #include <memory>
+#include <new>
 #include <string.h>
 
 namespace seera {
@@ -296,37 +297,44 @@ int adamw(bool eight, int count, float *const *w, const float *const *g, void *c
     if (total == 0) return SEERA_OK;
     ProfBytes pb((eight ? 12.0 + 2.0 * BLOCK_BYTES / BLOCK_ENTRIES : 28.0) * total, name);
     const void *kernel = eight ? (const void *)adamw8_kernel : (const void *)adamw_kernel;
-    auto table = std::make_shared<AdamWTable>();
+    AdamWTable table;
     AdamWArgs args = a;
     for (int i = 0; i < count;) {
-        memset(table.get(), 0, sizeof(AdamWTable));
-        table->hyper = hyper;
+        memset(&table, 0, sizeof table);
+        table.hyper = hyper;
         long long blocks = 0;
-        for (; i < count && table->count < TABLE; i++) {
+        for (; i < count && table.count < TABLE; i++) {
             if (n[i] == 0) continue;
             const long long need = (n[i] + CHUNK - 1) / CHUNK;
             if (blocks + need > 0x7fffffffLL) break;
-            table->first[table->count] = (unsigned)blocks;
-            table->decay[table->count] = decay[i];
-            AdamWTensor &t = table->t[table->count++];
+            table.first[table.count] = (unsigned)blocks;
+            table.decay[table.count] = decay[i];
+            AdamWTensor &t = table.t[table.count++];
             t.w = w[i]; t.g = g[i]; t.m = m[i]; t.n = n[i];
             if (eight) t.place = first;
             else t.v = v[i];
             blocks += need;
             if (eight) first += (n[i] + BLOCK_ENTRIES - 1) / BLOCK_ENTRIES * BLOCK_ENTRIES;
         }
-        if (!table->count) break;                             // tensors without entries were the last
-        void *argv[] = {table.get(), &args};
+        if (!table.count) break;                              // tensors without entries were the last
+        std::shared_ptr<void> kept;                           // a recorded launch's table, for other scalars
+        if (rt().capturing && !hyper) {
+            try {
+                kept = std::make_shared<AdamWTable>(table);
+            } catch (const std::bad_alloc &) {
+                return fail(SEERA_E_OOM, "%s: no host memory", name);
+            }
+        }
+        void *argv[] = {&table, &args};
         cudaLaunchKernel(kernel, dim3((unsigned)blocks), dim3(THREADS), argv, 0, rt().stream);
         SEERA_LAUNCH_CHECK(name);
-        if (rt().capturing && !hyper) {
+        if (kept) {
             OptLaunch l = {};
             l.kind = 2; l.grid = (int)blocks; l.n_scalars = eight ? 10 : 9;
             memcpy(l.scalars, &args, sizeof(float) * l.n_scalars);
             l.func = kernel;
-            l.table = table;
+            l.table = kept;
             if (int s = graph_note_optimizer(l)) return s;
-            table = std::make_shared<AdamWTable>();
         }
     }
     return SEERA_OK;

@@ -14,6 +14,7 @@
 #include <string>
 #include <map>
 #include <mutex>
+#include <new>
 #include <unordered_map>
 #include <vector>
 
@@ -162,8 +163,13 @@ int graph_note_optimizer(const OptLaunch &launch) {
     if (rt().graph_test_lose_update) n = 2;
     rt().graph_test_lose_update = false;                // one update only
     if (e == cudaSuccess && n == 1) {
-        p.cur->optimizers.push_back({deps[0], launch, p.cur->noted - 1});
-        return SEERA_OK;
+        try {
+            p.cur->optimizers.push_back({deps[0], launch, p.cur->noted - 1});
+            return SEERA_OK;
+        } catch (const std::bad_alloc &) {
+            p.cur->lost_update = true;
+            return fail(SEERA_E_OOM, "no host memory to note a recorded optimizer update");
+        }
     }
     cudaGetLastError();
     p.cur->lost_update = true;
