@@ -498,6 +498,9 @@ struct Resident { int clusters[MAX_RANKS + 1]; };
 // Blocks of a cluster: every cluster works through its tile's pieces one after the other, and the clusters that are not resident at once follow in
 // further rounds; the fewest pieces in a row win, and of equal sizes the smallest.  One sequence of 65536 steps and 512 channels, 16 tiles: 13 blocks take
 // 93 us; with every warp taking part in the exchange 13 took 111, 8 took 151, and 16, of which 14 clusters are resident, 145.
+// A block a tile where that leaves no place idle, whatever the count of pieces says: a cluster's blocks begin and end together and wait for one another.  512
+// sequences of 192 x 1024 take 329 us forward and 433 backward with one block, 513 forward with two; of 96 backward 304 and 503; 64 of 256 x 512 32 and 40 forward.  With few
+// tiles clusters win: 7 of 1024 x 645 backward 36 us, 41 with one block.
 template <int W, class P> int launch_scan(void (*kernel)(P), Resident &known, P p, int steps, int rows, const char *name) {
     const long long tiles = (long long)p.N * ((p.C + TILE - 1) / TILE);
     const size_t smem = (size_t)STAGES * W * rows * sizeof(float);
@@ -512,6 +515,7 @@ template <int W, class P> int launch_scan(void (*kernel)(P), Resident &known, P 
     attr[0].id = cudaLaunchAttributeClusterDimension;
     long long least = 0;
     for (int r = 1; r <= MAX_RANKS; r++) {
+        if (r > 1 && tiles >= known.clusters[1]) break;
         int &resident = known.clusters[r];
         if (!resident) {
             attr[0].val.clusterDim.x = (unsigned)r; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -562,8 +566,15 @@ template <bool VEC> __global__ void __launch_bounds__(256) pad_steps_kernel(cons
         }
     }
 }
-// Few steps: a thread per state has nothing to split.
-constexpr int SERIAL_STEPS = 16;
+// Whether the steps are few enough for a thread a state.  Those go at 0.27 us a step forward and 0.65 backward (two loads one after the other), and at the bytes' rate where states are many; the
+// split form takes what a round of its blocks takes, 2.4 us, two blocks an SM and a tile each, however few the steps of its first piece are.  So up to STEPS steps a round,
+// 9 forward and 4 backward; below a round's tenth the launch is all there is.  Thread a state against split, us forward / backward: 1 x 512 4 steps 7.1 / 8.2 against
+// 7.3 / 7.2, 16 steps 10 / 15 against 7 / 7; 8 x 2048 8 steps 9.1 / 11.3 against 11.3 / 11.2, 32 steps 15 / 28 against 11 / 11; 64 x 1024 16 steps 11 / 19 against
+// 22 / 24, 64 steps 28 / 56 against 27 / 32; 256 x 2048 16 steps 26 / 46 against 125 / 138, 64 steps 79 / 153 against 151 / 180.
+template <int STEPS> bool few_steps(int N, int T, int C, int at_least) {
+    const long long tiles = (long long)N * ((C + TILE - 1) / TILE);
+    return T <= at_least || T <= STEPS * tiles / (2 * rt().sm_count);
+}
 }  // namespace
 
 }  // namespace seera
@@ -580,7 +591,7 @@ int seera_gated_scan_fwd(const float *gate, const float *cand, int ld, const flo
     if (N == 0) return SEERA_OK;
     const ScanFwd p{gate, cand, h0, lengths, h, h_last, ld, N, T, C, 1, {}};
     ProfBytes pb((8.0 + (h ? 4 : 0)) * N * T * C, "gated_scan_fwd");
-    if (T <= SERIAL_STEPS) {
+    if (few_steps<9>(N, T, C, 4)) {
         scan_fwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("gated_scan_fwd");
         return SEERA_OK;
@@ -600,7 +611,7 @@ int seera_gated_scan_bwd(const float *gate, const float *cand, int ld, const flo
     if (N == 0) return SEERA_OK;
     const ScanBwd p{gate, cand, h0, lengths, h, dh, dh_last, dgate, dcand, dh0, ld, ld_grad, N, T, C, 1, {}};
     ProfBytes pb((20.0 + (dh ? 4 : 0)) * N * T * C, "gated_scan_bwd");
-    if (T <= SERIAL_STEPS) {
+    if (few_steps<4>(N, T, C, 2)) {
         scan_bwd_serial_kernel<<<(unsigned)(((long long)N * C + 127) / 128), 128, 0, rt().stream>>>(p);
         SEERA_LAUNCH_CHECK("gated_scan_bwd");
         return SEERA_OK;
