@@ -536,10 +536,13 @@ int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u,
  * seera_adamw8_step holds m and v in 8 bits: `state` of a tensor is seera_adamw8_state_bytes(n) bytes (8-byte aligned; zeros to start
  * with), 136 for each 64 neighbouring entries: sixteen times four codes of m and four of v, then the largest |m| and the largest v of the 64 as
  * floats.  A code times the block's largest is the entry: m has a sign, 4 bits of exponent and 3 of mantissa, v 5 bits of exponent and 3 of mantissa.
- * Rounding goes up or down at random with the value as its mean, but a v above zero never to 0 (2^-33 of its block's largest at least: the m beside it may
- * have been rounded up to 2^-17 of the largest, and m / sqrt(v) has no other bound); the random bits follow from `step` (the number of the step, a whole number below 2^24)
+ * Rounding goes up or down at random with the value as its mean; the random bits follow from `step` (the number of the step, a whole number below 2^24)
  * and the entry's place: `first`, a multiple of 64, plus its place in the tensors one after the other, each rounded up to 64.  w is updated from
  * m and v before they are rounded.  An infinity or a NaN in a gradient leaves none of the m and v of its 64 entries finite, where 32 bits would keep it to the one.
+ * Each average by itself keeps its mean, their quotient does not: where gradients within 64 entries are 2^-16 of the largest or less, an m that was rounded up may
+ * meet a v that was rounded to 0, and the step has no bound (1000 lr has been seen).  seera_adamw8_bounded_step is the same update on the same states, but a
+ * v above zero is held as 2^-33 of its block's largest at least: a step then stays near what 32 bits make of the same gradients, or is smaller.  It is what trains
+ * weights; seera_adamw8_step is for averages that have to keep their means down to the smallest, and keeps its results for the programs that call it.
  * seera_adamw8_read writes out the m and v that a state of n entries stands for. */
 int seera_adamw_step(int count, float *const *w, const float *const *g, float *const *m, float *const *v, const long long *n, const float *decay,
                      float lr, float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale,
@@ -548,6 +551,9 @@ size_t seera_adamw8_state_bytes(long long n);
 int seera_adamw8_step(int count, float *const *w, const float *const *g, void *const *state, const long long *n, const float *decay, float lr,
                       float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale, float step,
                       const float *hyper, long long first);
+int seera_adamw8_bounded_step(int count, float *const *w, const float *const *g, void *const *state, const long long *n, const float *decay, float lr,
+                              float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale, float step,
+                              const float *hyper, long long first);
 int seera_adamw8_read(const void *state, float *m, float *v, long long n);
 
 /* ---- data parallel: the gradient exchange of a batch sharded over the GPUs of one node -----------------------------

@@ -224,13 +224,17 @@ PYBIND11_MODULE(seera_cuda, m) {
     }, py::arg("w"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("n"), py::arg("decay"), py::arg("lr"), py::arg("beta1"), py::arg("omb1"), py::arg("beta2"),
        py::arg("omb2"), py::arg("eps"), py::arg("c1"), py::arg("c2"), py::arg("grad_scale"), py::arg("hyper") = 0);
     m.def("adamw8_state_bytes", [](long long n) { return seera_adamw8_state_bytes(n); });
-    m.def("adamw8_step", [](arr_p w, arr_p g, arr_p st, arr_l n, arr_f decay, float lr, float b1, float omb1, float b2, float omb2, float eps, float c1, float c2,
+    auto eight = [&m](const char *name, decltype(&seera_adamw8_step) entry) {
+        m.def(name, [entry](arr_p w, arr_p g, arr_p st, arr_l n, arr_f decay, float lr, float b1, float omb1, float b2, float omb2, float eps, float c1, float c2,
                             float gs, float step, uptr hyper, long long first) {
-        const py::ssize_t k = same_length({w.size(), g.size(), st.size(), n.size(), decay.size()});
-        ck(seera_adamw8_step((int)k, (F *const *)w.data(), (const F *const *)g.data(), (void *const *)st.data(), n.data(), decay.data(), lr, b1, omb1, b2,
-                             omb2, eps, c1, c2, gs, step, P<const F>(hyper), first));
-    }, py::arg("w"), py::arg("g"), py::arg("state"), py::arg("n"), py::arg("decay"), py::arg("lr"), py::arg("beta1"), py::arg("omb1"), py::arg("beta2"),
-       py::arg("omb2"), py::arg("eps"), py::arg("c1"), py::arg("c2"), py::arg("grad_scale"), py::arg("step"), py::arg("hyper") = 0, py::arg("first") = 0);
+            const py::ssize_t k = same_length({w.size(), g.size(), st.size(), n.size(), decay.size()});
+            ck(entry((int)k, (F *const *)w.data(), (const F *const *)g.data(), (void *const *)st.data(), n.data(), decay.data(), lr, b1, omb1, b2,
+                     omb2, eps, c1, c2, gs, step, P<const F>(hyper), first));
+        }, py::arg("w"), py::arg("g"), py::arg("state"), py::arg("n"), py::arg("decay"), py::arg("lr"), py::arg("beta1"), py::arg("omb1"), py::arg("beta2"),
+              py::arg("omb2"), py::arg("eps"), py::arg("c1"), py::arg("c2"), py::arg("grad_scale"), py::arg("step"), py::arg("hyper") = 0, py::arg("first") = 0);
+    };
+    eight("adamw8_step", seera_adamw8_step);
+    eight("adamw8_bounded_step", seera_adamw8_bounded_step);
     m.def("adamw8_read", [](uptr st, uptr mm, uptr v, long long n) { ck(seera_adamw8_read(P<const void>(st), P<F>(mm), P<F>(v), n)); });
 
     m.def("cuda_adam_step_dev", [](uptr w, uptr g, uptr mm, uptr v, int n, uptr h) {

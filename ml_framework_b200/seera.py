@@ -1997,7 +1997,7 @@ class AdamW(_Optimizer):
     """Adam with decoupled weight decay: w = (1 - lr weight_decay) w - lr (m / c1) / (sqrt(v / c2) + eps).  The layers' weight matrices and
     filters decay; biases and the factors of norms do not.  A recorded step keeps the weight_decay that it was recorded with (lr and the rest follow).
 
-    state_bits  32, or 8: m and v in 8 bits each with a largest value per 64 entries, 2.125 bytes a parameter instead of 8 (see seera_adamw8_step)."""
+    state_bits  32, or 8: m and v in 8 bits each with a largest value per 64 entries, 2.125 bytes a parameter instead of 8 (see seera_adamw8_bounded_step)."""
 
     def __init__(self, model, lr=0.001, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32):
         super().__init__(model)
@@ -2054,4 +2054,4 @@ class AdamW(_Optimizer):
         if self.state_bits == 32:
             sc.adamw_step(*table, *(scalars or [0.0] * 9), hyper=hyper)
         else:
-            sc.adamw8_step(*table, *(scalars or [0.0] * 10), hyper=hyper, first=begin)
+            sc.adamw8_bounded_step(*table, *(scalars or [0.0] * 10), hyper=hyper, first=begin)

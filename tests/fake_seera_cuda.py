@@ -692,8 +692,14 @@ def adamw_step(w, g, m, v, n, decay, *s, hyper=0):
 def adamw8_state_bytes(n): return -(-n // 64) * 136
 
 
-def adamw8_step(w, g, state, n, decay, *s, hyper=0, first=0):
+def adamw8_step(w, g, state, n, decay, *s, hyper=0, first=0): _adamw8("pack8", w, g, state, n, decay, s, hyper, first)
+def adamw8_bounded_step(w, g, state, n, decay, *s, hyper=0, first=0): _adamw8("bounded", w, g, state, n, decay, s, hyper, first)
+
+
+def _adamw8(rule, w, g, state, n, decay, s, hyper, first):
+    import adamw8_np
     import sequence_np as ref
+    pack = ref.pack8 if rule == "pack8" else adamw8_np.pack8_bounded
     _count("adamw8")
     s = _adamw_scalars(s, hyper, 10)
     for W, G, S, k, d in zip(*(np.asarray(a).tolist() for a in (w, g, state, n, decay))):
@@ -701,5 +707,5 @@ def adamw8_step(w, g, state, n, decay, *s, hyper=0, first=0):
         m, v = ref.unpack8(st, k)
         a, b, c, _ = ref.adamw(_view(W, k), _view(G, k), m, v, d, *s[:9])
         _view(W, k)[:] = a
-        st[:] = ref.pack8(b, c, int(s[9]), first)
+        st[:] = pack(b, c, int(s[9]), first)
         first += -(-k // 64) * 64

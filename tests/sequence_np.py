@@ -212,7 +212,6 @@ def pack8(m, v, step, first=0):
         im, iv = (np.where(a > 0, np.float32(1) / a, np.float32(0)).astype(np.float32)[:, None] for a in (am, av))
         cm = _codes(np.abs(M), im, 2.0 ** -112, 0x78, r & np.uint64(0xFFFF)) | np.where(M < 0, np.uint32(128), np.uint32(0))
         cv = _codes(V, iv, 2.0 ** -96, 0xF8, r >> np.uint64(16))
-        cv = np.maximum(cv, (V > 0) & (av > 0)[:, None] & np.isfinite(av)[:, None])             # a v above zero is not held as 0
     out = np.zeros((blocks, 136), np.uint8)
     body = out[:, :128].reshape(-1, 16, 2, 4)
     body[:, :, 0], body[:, :, 1] = cm.reshape(-1, 16, 4), cv.reshape(-1, 16, 4)

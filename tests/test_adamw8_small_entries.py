@@ -10,7 +10,9 @@ import ctypes
 import numpy as np
 import pytest
 
+import adamw8_np
 import sequence_np as ref
+from test_host_logic_cpu import host  # noqa: F401  (fixture)
 
 LARGEST, RMS = 7.3 + 5.0, 1.3
 B1, B2, STEPS, BLOCKS = 0.9, 0.999, 300, 16
@@ -36,7 +38,7 @@ def model(g, eight):
     for t, x in enumerate(g, 1):
         move, m, v, _ = ref.adamw(w, x, m, v, 0.0, *hp(t))
         if eight:
-            m, v = ref.unpack8(ref.pack8(m, v, t), n)
+            m, v = ref.unpack8(adamw8_np.pack8_bounded(m, v, t), n)
         moves.append(move)
     return np.array(moves)
 
@@ -61,13 +63,36 @@ def test_rule_keeps_the_steps(e, scale, mean):
 def test_what_the_rule_leaves_zero():
     """A v of 0, and all of a block whose largest is held as 0 or is not finite."""
     m = np.ones(64, np.float32)
-    code = lambda v: ref.pack8(m, v, 5)[:128].reshape(16, 2, 4)[:, 1].reshape(-1)  # noqa: E731
+    code = lambda v: adamw8_np.pack8_bounded(m, v, 5)[:128].reshape(16, 2, 4)[:, 1].reshape(-1)  # noqa: E731
     v = np.full(64, 1e-30, np.float32)
     v[0], v[1] = 1.0, 0.0
     assert code(v)[0] == 0xF8 and code(v)[1] == 0 and (code(v)[2:] == 1).all()
     assert (code(np.full(64, 1e-40, np.float32)) == 0).all()
     v[0] = np.inf
     assert (code(v)[1:] == 0).all()
+
+
+def test_optimizer_takes_bounded_steps(host, monkeypatch):
+    """A model whose gradients have entries 2^-17 and 2^-20 of their neighbours, through AdamW itself."""
+    S = host.seera
+    monkeypatch.setattr(host.fake, "adamw8_step", None)
+    model = S.Sequential([S.Input((64,)), S.Dense(64, 8, "tanh"), S.Dense(8, 4, "tanh")])
+    r = np.random.RandomState(2)
+    X = r.standard_normal((16, 64)).astype(np.float32) * np.float32(2.0) ** -np.array([0, 17, 17, 20] * 16, np.float32)
+    w = model.param_layers[0].weights
+    moves = {}
+    for bits in (32, 8):
+        model.param_layers[0].set_weights(np.zeros((64, 8), np.float32), np.zeros((1, 8), np.float32))
+        opt, moves[bits] = S.AdamW(model, lr=2.0 ** -20, weight_decay=0.0, state_bits=bits), []
+        for _ in range(120):
+            Y = r.standard_normal((16, 4)).astype(np.float32) * 30
+            S.autograd4nn(S.Loss().mse(model.forward(X), S.Tensor(Y, is_leaf=True)))
+            before = w.to_numpy().astype(np.float64)
+            opt.step()
+            model.zero_grad()
+            moves[bits].append((w.to_numpy() - before) * 2.0 ** 20)
+    assert np.abs(moves[32]).max() < 7.4
+    assert np.abs(moves[8]).max() <= LARGEST
 
 
 @pytest.mark.gpu
@@ -82,7 +107,7 @@ def test_kernel_keeps_the_steps(e, scale, mean):
         st = d.up(np.zeros(d.L.seera_adamw8_state_bytes(n), np.uint8), np.uint8)
         pw, pg = [d.up(np.zeros(n, np.float32)) for _ in g], [d.up(x) for x in g]
         for t in range(1, STEPS + 1):
-            capi.check(d.L.seera_adamw8_step(1, one(pw[t - 1]), one(pg[t - 1]), one(st), (ctypes.c_longlong * 1)(n), (ctypes.c_float * 1)(0.0), *hp(t), float(t),
+            capi.check(d.L.seera_adamw8_bounded_step(1, one(pw[t - 1]), one(pg[t - 1]), one(st), (ctypes.c_longlong * 1)(n), (ctypes.c_float * 1)(0.0), *hp(t), float(t),
                                              None, 0))
         moves = np.array([d.down(p, (n,)) for p in pw], np.float64)
     a = small(moves)
@@ -111,12 +136,30 @@ def test_kernel_leaves_zero_what_the_rule_does():
         m, v = np.zeros(n, np.float32), np.zeros(n, np.float32)
         for t in (1, 2, 3):
             h = (lr,) + hp(t)[1:]
-            capi.check(d.L.seera_adamw8_step(1, one(pw), one(pg), one(st), (ctypes.c_longlong * 1)(n), (ctypes.c_float * 1)(0.0), *h, float(t), None, 0))
+            capi.check(d.L.seera_adamw8_bounded_step(1, one(pw), one(pg), one(st), (ctypes.c_longlong * 1)(n), (ctypes.c_float * 1)(0.0), *h, float(t), None, 0))
             _, m, v, _ = ref.adamw(np.zeros(n, np.float32), g, m, v, 0.0, *h)
-            packed = ref.pack8(m, v, t)
+            packed = adamw8_np.pack8_bounded(m, v, t)
             got = d.down(st, (nb,), np.uint8)
             top = lambda s: np.ascontiguousarray(s.reshape(-1, 136)[:, 128:]).view(np.float32)  # noqa: E731
             finite = np.isfinite(top(packed)).all(1)
             assert np.array_equal(got.reshape(-1, 136)[finite], packed.reshape(-1, 136)[finite])
             assert np.array_equal(np.isfinite(top(got)).all(1), finite) and finite.sum() == 5
             m, v = ref.unpack8(packed, n)
+
+
+@pytest.mark.gpu
+def test_refusals():
+    from ml_framework_b200 import capi
+    import engine_np
+    n = 100
+    with engine_np._Dev() as d:
+        w, g, st = d.up(np.arange(n, dtype=np.float32)), d.up(np.ones(n, np.float32)), d.up(np.zeros(2 * 136, np.uint8), np.uint8)
+        one = lambda q: (ctypes.c_void_p * 1)(q)  # noqa: E731
+        call = lambda w, g, s, k, step, first: d.L.seera_adamw8_bounded_step(1, one(w), one(g), one(s), (ctypes.c_longlong * 1)(k), (ctypes.c_float * 1)(0.0), *hp(1),  # noqa: E731
+                                                                             step, None, first)
+        launches = d.L.seera_launch_count()
+        for bad in ((None, g, st, n, 1.0, 0), (w, None, st, n, 1.0, 0), (w, g, None, n, 1.0, 0), (w, g, st + 4, n, 1.0, 0), (w, g, st, -1, 1.0, 0),
+                    (w, g, st, n, -1.0, 0), (w, g, st, n, float("nan"), 0), (w, g, st, n, 1.0, -64), (w, g, st, n, 1.0, 32), (w, g, st, (1 << 40) + 1, 1.0, 0)):
+            assert call(*bad) != 0
+        assert call(w, g, st, 0, 1.0, 0) == 0
+        assert d.L.seera_launch_count() == launches and np.array_equal(d.down(w, (n,)), np.arange(n))
