@@ -15,10 +15,10 @@
 // registers (first the mean, then the differences to it), sums in fp32 by halves.
 // Sums over the rows: a thread always has the same columns, so it adds up its part in registers; a block writes its sums once, and a last launch adds
 // the blocks' in a fixed order: the same bits on every run.
-// The backward kernels and the plain norm run as many blocks as are resident, each with the next rows on their way while it works on one: what is left
-// to wait for are two sums over the block's threads a row.  Measured (fp32, inputs beyond L2): norm of 16384 x 1280 31 us forward and 44 backward (5.1
-// TB/s) with 7 for the sums over the blocks; residual of 16384 x 2048 117 us forward (5.7 TB/s) and 208 backward (5.1 TB/s).  Loads straight into
-// registers, two blocks an SM and sums in shared memory took 297 for the last.
+// The backward kernels and the plain norm run as many blocks as are resident, each with the next row on its way while it works on one: what is left
+// to wait for are two sums over the block's threads a row.  Measured (fp32, inputs beyond L2): norm of 16384 x 1280 both ways 82 us, 6 of them for the sums over
+// the blocks (5.4 TB/s in the backward kernel); residual of 16384 x 2048 119 us forward (5.6 TB/s) and 201 backward (5.3 TB/s), the same with the gate as a range of wider
+// rows.  Loads straight into registers, two blocks an SM and sums in shared memory took 297 for the last.
 #include "common.cuh"
 #include "internal.h"
 #include "sigmoid.cuh"
