@@ -541,8 +541,9 @@ int seera_gated_residual_bwd(const float *dout, const float *dy, const float *u,
  * m and v before they are rounded.  An infinity or a NaN in a gradient leaves none of the m and v of its 64 entries finite, where 32 bits would keep it to the one.
  * Each average by itself keeps its mean, their quotient does not: where gradients within 64 entries are 2^-16 of the largest or less, an m that was rounded up may
  * meet a v that was rounded to 0, and the step has no bound (1000 lr has been seen).  seera_adamw8_bounded_step is the same update on the same states, but a
- * v above zero is held as 2^-33 of its block's largest at least: a step then stays near what 32 bits make of the same gradients, or is smaller.  It is what trains
- * weights; seera_adamw8_step is for averages that have to keep their means down to the smallest, and keeps its results for the programs that call it.
+ * v above zero is held as 2^-33 of its block's largest at least: a step then stays near what 32 bits make of the same gradients, or is smaller (on states
+ * that it has written: the first one on another's may still be such a step).  It is what trains weights; seera_adamw8_step is for averages that have to keep
+ * their means down to the smallest, and keeps its results for the programs that call it.
  * seera_adamw8_read writes out the m and v that a state of n entries stands for. */
 int seera_adamw_step(int count, float *const *w, const float *const *g, float *const *m, float *const *v, const long long *n, const float *decay,
                      float lr, float beta1, float omb1, float beta2, float omb2, float eps, float c1, float c2, float grad_scale,
